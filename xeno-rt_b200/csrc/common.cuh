@@ -163,12 +163,11 @@ template <> __device__ __forceinline__ float swish_for<__nv_bfloat16>(float x, f
   return __fdividef(x, 1.0f + __expf(-alpha * x));
 }
 
-// COUNT hidden units of a gated feed-forward from the two sums of their row pairs, as RowScale says, into g: units n,
-// n + 1, .. with ALONG, else COUNT times unit n (of several tokens).  The kind of gate is chosen once for all of them, so
-// that their exponentials and divisions run side by side.  Units at or beyond gate_up (with biases: the product's
-// width) are not stored by anybody: they get some other unit's biases.
-template <typename TO, int COUNT, bool ALONG>
-__device__ __forceinline__ void gated_units(float (&g)[COUNT], float (&u)[COUNT], int n, const RowScale& s) {
+// Adds the biases of COUNT hidden units to the two sums of their row pairs (RowScale): units n, n + 1, .. with ALONG, else
+// COUNT times unit n.  Units at or beyond gate_up (with biases: the product's width) are not stored by anybody: they get
+// some other unit's biases.
+template <int COUNT, bool ALONG>
+__device__ __forceinline__ void add_gate_biases(float (&g)[COUNT], float (&u)[COUNT], int n, const RowScale& s) {
   if (s.gate_bias != nullptr) {
     const float* up = s.gate_bias + s.gate_up;
     if (!ALONG) {
@@ -193,6 +192,14 @@ __device__ __forceinline__ void gated_units(float (&g)[COUNT], float (&u)[COUNT]
       }
     }
   }
+}
+
+// COUNT hidden units of a gated feed-forward from the two sums of their row pairs, as RowScale says, into g: units n,
+// n + 1, .. with ALONG, else COUNT times unit n (of several tokens).  The kind of gate is chosen once for all of them, so
+// that their exponentials and divisions run side by side.
+template <typename TO, int COUNT, bool ALONG>
+__device__ __forceinline__ void gated_units(float (&g)[COUNT], float (&u)[COUNT], int n, const RowScale& s) {
+  add_gate_biases<COUNT, ALONG>(g, u, n, s);
   if (s.gate_act == 2) {
     const float limit = s.gate_limit, alpha = s.gate_alpha;
 #pragma unroll

@@ -91,6 +91,10 @@ _SIGNATURES = {
     "xrt_recurrence_gates": [_P, _P, _P, _P, _P, _I, _P],
     "xrt_recurrence_scan": [_P, _P, _I, _I, _P],
     "xrt_recurrence_step": [_P, _P, _P, _P, _P, _P, _I, _P],
+    "xrt_quantize_rows": [_P, _P, _P, _I, _I, _I, _I, _P],
+    "xrt_swiglu_int8": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P],
+    "xrt_rmsnorm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _P],
+    "xrt_gemm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "xrt_fill_normal": [_P, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_double, _I, _P],
     "xrt_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P],
     "xrt_mark_seen": [_P, _I, _P, _P, _I, _I, _P],
@@ -1688,3 +1692,127 @@ def linear_recurrence_step(out, p, w: RecurrenceWeights, state, ring, tok_slot, 
     _check(_kernels().xrt_recurrence_step(_ptr(out, "out", torch.bfloat16), args, _ptr(w.r, "r", torch.bfloat16),
                                           _ptr(w.i, "i", torch.bfloat16), _ptr(tok_slot, "tok_slot", torch.int32),
                                           _ptr(tok_pos, "tok_pos", torch.int32), n, _stream()), "recurrence_step")
+
+
+# ------------------------------------------------------------------ products of 8-bit integers
+INT8_MAX_INPUTS = 131071  # 128 * 128 * K stays below 2^31
+
+
+def int8_rows(rows: int, width: int, device) -> torch.Tensor:
+    """An int8 tensor [rows, width], not filled, whose rows begin every 16 bytes, as ``gemm_int8`` asks for."""
+    return torch.empty((rows, -(-width // 16) * 16), dtype=torch.int8, device=device)[:, :width]
+
+
+def _launch_on(what: str, tensors, call) -> None:
+    """``call(stream)`` on the one device that all of ``tensors`` (None: not given) lie on, whichever is current."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise KernelError(f"{what}: all tensors must be on one CUDA device")
+    lib = _kernels()
+    if device.index == torch.cuda.current_device():
+        _check(call(lib, torch.cuda.current_stream(device).cuda_stream), what)
+    else:
+        with torch.cuda.device(device):
+            _check(call(lib, torch.cuda.current_stream(device).cuda_stream), what)
+
+
+def _error_flag_pointer(device) -> int:
+    """The device's error flag for a launch; 0 (the kernel reports nothing) where it would have to be made inside a capture."""
+    if device.index not in _error_flags and torch.cuda.is_current_stream_capturing():
+        return 0
+    return error_flag(device).data_ptr()
+
+
+def _codes(t, name: str, what: str, rows: int, width: int) -> int:
+    """The distance of the rows of an int8 tensor [rows, width] in bytes."""
+    if t.dtype != torch.int8 or tuple(t.shape) != (rows, width):
+        raise KernelError(f"{what}: {name} must be int8 [{rows}, {width}], not {t.dtype} {tuple(t.shape)}")
+    if (width > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < width):
+        raise KernelError(f"{what}: the rows of {name} must be contiguous")
+    return t.stride(0) if rows > 1 else -(-width // 16) * 16
+
+
+def _vector(t, name: str, what: str, size: int) -> int:
+    if t.dtype != torch.float32 or tuple(t.shape) != (size,) or not t.is_contiguous():
+        raise KernelError(f"{what}: {name} must be float32 [{size}] without gaps, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def quantize_rows(codes, scales, x) -> None:
+    """Every row of ``x`` (float32 or bfloat16 [n, width]) as 8-bit integers with one scale: scales[r] = max(max |x[r]| / 127,
+    2^-126), codes[r] = x[r] / scales[r] rounded to the nearest (ties to even).  ``codes`` int8 [n, width], rows contiguous
+    (``int8_rows`` makes one that ``gemm_int8`` takes); ``scales`` float32 [n].  A row with a NaN or an infinity
+    gets codes 0 and the scale NaN."""
+    what = "quantize_rows"
+    if x.dim() != 2:
+        raise KernelError(f"{what}: x must be [rows, width]")
+    n, width = x.shape
+    ld = _codes(codes, "codes", what, n, width)
+    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), n, width, ld, _code(x.dtype))
+    _launch_on(what, (x, codes, scales), lambda lib, stream: lib.xrt_quantize_rows(*args, stream))
+
+
+def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
+    """``swiglu`` with its result as 8-bit integers: codes[t], scales[t] are ``quantize_rows`` of act(gate_up[t, :F]) *
+    gate_up[t, F:], which is 32-bit and not written.  ``gate_up`` float32 or bfloat16 [n, 2 * F]; ``act`` "silu" or "gelu_tanh",
+    or a ``Gate`` (a limited gate, biases)."""
+    what = "swiglu_int8"
+    gate = _gate_of(act)
+    code = _gate_code(gate, "swiglu")
+    if gate_up.dim() != 2 or gate_up.shape[1] % 2:
+        raise KernelError(f"{what}: gate_up must be [rows, 2 * width]")
+    n, width = gate_up.shape[0], gate_up.shape[1] // 2
+    ld = _codes(codes, "codes", what, n, width)
+    options = gate.options(width)
+    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), n, width, ld, _code(gate_up.dtype),
+            code, options)
+    _launch_on(what, (gate_up, codes, scales, gate.bias), lambda lib, stream: lib.xrt_swiglu_int8(*args, stream))
+
+
+def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None) -> None:
+    """The RMSNorm of the residual stream as 8-bit integers, something added to the stream on the way: s = x + add (``add``
+    float32 or bfloat16 [n, width], or None: s = x), written to ``out`` (float32 [n, width]; None: into ``x``); codes[r],
+    scales[r] are ``quantize_rows`` of s[r] / sqrt(mean(s[r]^2) + eps) * weight, which is 32-bit and not written.  ``x``
+    float32 [n, width], ``weight`` float32 or bfloat16 [width]."""
+    what = "rmsnorm_int8"
+    if x.dim() != 2 or tuple(weight.shape) != (x.shape[1],):
+        raise KernelError(f"{what}: x must be [rows, width] and weight [width]")
+    if add is None and out is not None:
+        raise KernelError(f"{what}: out is the sum of x and add, and there is no add")
+    n, width = x.shape
+    if add is not None:
+        out = x if out is None else out
+        if add.shape != x.shape or out.shape != x.shape:
+            raise KernelError(f"{what}: add and out must have the shape of x")
+    ld = _codes(codes, "codes", what, n, width)
+    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),
+            _ptr(out, "out", torch.float32), _ptr(weight, "weight"), n, width, ld, float(eps),
+            0 if add is None else _code(add.dtype), _code(weight.dtype))
+    _launch_on(what, (x, codes, scales, weight, add, out), lambda lib, stream: lib.xrt_rmsnorm_int8(*args, stream))
+
+
+def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = False, bias=None) -> None:
+    """out[m, n] = scales[m] * weight_scales[n] * sum_k codes[m, k] * weight[n, k] (+ bias[n]), or added into a float32 ``out``
+    with ``accumulate``.  ``codes`` int8 [M, K] and ``weight`` int8 [N, K], rows beginning every so many 16 bytes (``int8_rows``;
+    what lies between the rows is not read); the sum is exact (K up to ``INT8_MAX_INPUTS``), the rest 32-bit.
+    ``scales`` [M], ``weight_scales`` and ``bias`` [N] float32; ``out`` float32 or bfloat16 [M, N], its rows contiguous."""
+    what = "gemm_int8"
+    if codes.dim() != 2 or weight.dim() != 2 or codes.shape[1] != weight.shape[1]:
+        raise KernelError(f"{what}: shapes do not fit: codes {tuple(codes.shape)}, weight {tuple(weight.shape)}")
+    (m, k), n = codes.shape, weight.shape[0]
+    if k > INT8_MAX_INPUTS:
+        raise KernelError(f"{what}: sums over {k} inputs can pass 32 bits; at most {INT8_MAX_INPUTS} are taken")
+    ldx, ldw = _codes(codes, "codes", what, m, k), _codes(weight, "weight", what, n, k)
+    for name, t, ld in (("codes", codes, ldx), ("weight", weight, ldw)):
+        if ld % 16 or t.data_ptr() % 16:
+            raise KernelError(f"{what}: the rows of {name} must begin every so many 16 bytes (see int8_rows)")
+    if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        raise KernelError(f"{what}: out must be [{m}, {n}] with contiguous rows")
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError(f"{what}: only a float32 out is added into")
+    args = (out.data_ptr(), codes.data_ptr(), _vector(scales, "scales", what, m), weight.data_ptr(),
+            _vector(weight_scales, "weight_scales", what, n), 0 if bias is None else _vector(bias, "bias", what, n), m, n, k,
+            ldx, ldw, out.stride(0) if m > 1 else n, _code(out.dtype), 1 if accumulate else 0)
+    _launch_on(what, (out, codes, scales, weight, weight_scales, bias),
+               lambda lib, stream: lib.xrt_gemm_int8(*args, _error_flag_pointer(out.device), stream))

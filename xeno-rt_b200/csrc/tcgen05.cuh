@@ -1,8 +1,8 @@
 // The Blackwell (sm_100a) instructions that the tensor-core kernels of this library share, as thin
 // wrappers over inline PTX: mbarriers with bounded waits, TMA tensor copies, shared-memory and
 // instruction descriptors of tcgen05.mma (kind::f16, bfloat16 operands, float32 accumulators in tensor
-// memory), commits, fences, tensor-memory loads and stores, and the driver's tensor-map encoder.
-// Used by gemm_tcgen05.cu (prompt products), gemm_decode_tcgen05.cu (few-row products), moe_grouped.cu (experts'
+// memory; kind::i8, 8-bit and 32-bit integers), commits, fences, tensor-memory loads and stores, and the driver's tensor-map encoder.
+// Used by gemm_tcgen05.cu (prompt products), gemm_decode_tcgen05.cu (few-row products), gemm_int8.cu (8-bit products), moe_grouped.cu (experts'
 // products) and attention_prefill_tcgen05.cu (prompt attention).
 #pragma once
 
@@ -125,6 +125,22 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t desc_a, u
                " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
                ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// kind::i8: D (32-bit integers in tensor memory) = A . B or += A . B of signed 8-bit integers, both K-major, 32 bytes of the
+// contraction an instruction.  Instruction descriptor: 32-bit integer D (2 in bits [4, 6)), signed A (1 in bits [7, 10)) and
+// B (1 in bits [10, 13)), no saturation, N / 8 in bits [17, 23), M / 16 in bits [24, 29).
+__host__ __device__ constexpr uint32_t instr_desc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
+               ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
+               ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
 // One arrival on the barrier at this place in BOTH blocks when every MMA of the pair issued so far has completed.
 __device__ __forceinline__ void commit_pair(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
@@ -191,6 +207,20 @@ inline bool make_map_bf16_2d(CUtensorMap* map, const void* base, long long rows,
   const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
   const cuuint32_t elem[2] = {1u, 1u};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The same over 8-bit integers [rows, cols] with row stride `ld` bytes (a multiple of 16): boxes of `box_rows` rows x 128
+// columns.  What a box has beyond rows or cols arrives as zeros.
+inline bool make_map_int8_2d(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_rows) {
+  TensorMapEncodeFn encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1u, 1u};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

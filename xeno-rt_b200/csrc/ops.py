@@ -94,7 +94,7 @@ _SIGNATURES = {
     "xrt_quantize_rows": [_P, _P, _P, _I, _I, _I, _I, _P],
     "xrt_swiglu_int8": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P],
     "xrt_rmsnorm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _P],
-    "xrt_gemm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "xrt_gemm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "xrt_fill_normal": [_P, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_double, _I, _P],
     "xrt_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P],
     "xrt_mark_seen": [_P, _I, _P, _P, _I, _I, _P],
@@ -1792,11 +1792,14 @@ def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None) -> No
     _launch_on(what, (x, codes, scales, weight, add, out), lambda lib, stream: lib.xrt_rmsnorm_int8(*args, stream))
 
 
-def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = False, bias=None) -> None:
+def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = False, bias=None,
+              constant_weight: bool = False) -> None:
     """out[m, n] = scales[m] * weight_scales[n] * sum_k codes[m, k] * weight[n, k] (+ bias[n]), or added into a float32 ``out``
     with ``accumulate``.  ``codes`` int8 [M, K] and ``weight`` int8 [N, K], rows beginning every so many 16 bytes (``int8_rows``;
     what lies between the rows is not read); the sum is exact (K up to ``INT8_MAX_INPUTS``), the rest 32-bit.
-    ``scales`` [M], ``weight_scales`` and ``bias`` [N] float32; ``out`` float32 or bfloat16 [M, N], its rows contiguous."""
+    ``scales`` [M], ``weight_scales`` and ``bias`` [N] float32; ``out`` float32 or bfloat16 [M, N], its rows contiguous.  ``constant_weight``: the
+    weight is a model's, which no kernel that may still run has written: products of few rows then read it while the
+    kernel before them finishes."""
     what = "gemm_int8"
     if codes.dim() != 2 or weight.dim() != 2 or codes.shape[1] != weight.shape[1]:
         raise KernelError(f"{what}: shapes do not fit: codes {tuple(codes.shape)}, weight {tuple(weight.shape)}")
@@ -1813,6 +1816,6 @@ def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = Fals
         raise KernelError(f"{what}: only a float32 out is added into")
     args = (out.data_ptr(), codes.data_ptr(), _vector(scales, "scales", what, m), weight.data_ptr(),
             _vector(weight_scales, "weight_scales", what, n), 0 if bias is None else _vector(bias, "bias", what, n), m, n, k,
-            ldx, ldw, out.stride(0) if m > 1 else n, _code(out.dtype), 1 if accumulate else 0)
+            ldx, ldw, out.stride(0) if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0)
     _launch_on(what, (out, codes, scales, weight, weight_scales, bias),
                lambda lib, stream: lib.xrt_gemm_int8(*args, _error_flag_pointer(out.device), stream))

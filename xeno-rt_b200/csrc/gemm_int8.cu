@@ -12,6 +12,8 @@
 //              patch around in shared memory and stores 16 bytes a lane, while the MMA warp fills the other accumulator.
 // Every wait on an mbarrier is bounded.  A wait that runs out raises the error flag and an abort flag in shared memory; all
 // roles leave their loops, the block frees its TMEM and returns.
+#include <type_traits>
+
 #include "tcgen05.cuh"
 
 namespace xrt {
@@ -71,7 +73,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 
   bool ok = true;
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int it = 0;
       for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
         const int m0 = tile % tiles_m * I8_BM, n0 = tile / tiles_m * I8_BN;
@@ -88,7 +90,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = instr_desc_i8(I8_BM, I8_BN);
       int it = 0, tile_i = 0;
       for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x, ++tile_i) {
@@ -159,7 +161,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       mbar_arrive(smem_u32(&acc_empty[a]));
     }
   }
-  if (!ok && lane == 0) { *abort_flag = 1; if (error_flag != nullptr) atomicExch(error_flag, 6); }
+  if (!ok) { *abort_flag = 1; if (error_flag != nullptr) atomicExch(error_flag, 6); }
 
   fence_before();
   __syncthreads();
@@ -182,34 +184,49 @@ int launch_gemm_int8(void* out, const CUtensorMap& map_x, const CUtensorMap& map
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to 128 rows the operands are swapped: 128 WEIGHT rows are the MMA's lanes and the rows of codes its N (16 .. 128), and the
-// time is the time to stream W from memory.  A block takes one tile of 128 weight rows and one of `splits` parts of K; the
-// parts of a tile are the blocks of a cluster.  Two blocks a multiprocessor are resident (their rings are cut to fit), so
-// that the copies of one run while the other starts or finishes, and all of a product's blocks together hold many
-// times the bytes in flight that the memory needs.  Every block sends its sums for a share of the tile's rows to the block
+// Up to 128 rows the operands are swapped: WEIGHT rows are the MMA's lanes and the rows of codes its N (16 .. 128), and the
+// time is the time to stream W from memory and through every multiprocessor's port to the L2.  A block takes a tile of
+// any number of weight rows up to 256 (one or two MMAs; lanes beyond the tile's rows hold whatever lies behind them in shared
+// memory and are never read) and one of `splits` parts of K, so that every multiprocessor gets the same share of W.  The
+// parts of a tile are the blocks of a cluster: every block sends its sums for a share of the tile's rows to the block
 // that finishes them (remote stores into shared memory that no ring uses), the cluster meets once, and every block adds its
 // rows' sums: whole numbers, so their order does not matter.
-constexpr int FEW_MAX_ROWS = 128, FEW_MAX_SPLITS = 8;
-constexpr int FEW_W_BYTES = 128 * I8_BK;
-constexpr int FEW_THREADS = 192;
-constexpr int FEW_TAIL_BYTES = 512;  // barriers and flags
+//
+// Nine warps: warps 0-3 issue the copies, every fourth slab of K each, because the copies of one warp run few at a
+// time (measured with boxes of 128 rows x 128 bytes from memory, GB/s into one multiprocessor: one warp 55, two 98, four 127);
+// warp 4 owns the TMEM and issues the MMAs; warps 5-8 bring the accumulators to shared memory, where all warps finish them.  A
+// kernel this short also pays for every instruction that it meets for the first time (its code comes from the L2): the
+// finish is one short loop, and while warps 5-8 wait they walk it once into a place that nobody reads.
+constexpr int FEW_MAX_ROWS = 128, FEW_MAX_SPLITS = 8, FEW_MAX_STAGES = 24;
+constexpr int FEW_PRODUCERS = 4;
+constexpr int FEW_THREADS = 32 * (FEW_PRODUCERS + 1 + 4);
+constexpr int FEW_TAIL_BYTES = 512 + 4 * (FEW_MAX_ROWS + 2 * 256);  // barriers, flags, a place that nobody reads; scales, biases
 
 struct FewShape {
   int M, N, ldo;
-  int nb;       // rows of codes, padded to a multiple of 16
-  int splits, stages;
-  int k_iters;  // slabs of 128 of K
-  int early;    // the weight may be read before the kernel before this one is done
+  int nb;        // rows of codes, padded to a multiple of 16
+  int rows;      // weight rows of a tile
+  int splits;
+  int slabs;     // of 128 of K in a stage: 1, 2 or 4
+  int stages;
+  int k_iters;   // stages' worth of K
+  int early;     // the weight may be read before the kernel before this one is done
 };
 
-__host__ __device__ inline int few_stage_bytes(int nb) { return FEW_W_BYTES + nb * I8_BK; }
+__host__ __device__ inline int few_w_bytes(const FewShape& s) { return (s.rows * I8_BK + 1023) & ~1023; }  // of a slab
+__host__ __device__ inline int few_stage_bytes(const FewShape& s) { return s.slabs * (few_w_bytes(s) + s.nb * I8_BK); }
 // Weight rows that one block of a cluster finishes; the last has the remainder.
-__host__ __device__ inline int few_rows_per_block(int splits) { return ((128 + splits - 1) / splits + 3) & ~3; }
-
-template <int MODE, typename TO>
-__device__ __forceinline__ void few_store(TO* dst, int sum, float row_scale, float column_scale, float bias) {
-  const float value = fmaf(__int2float_rn(sum) * row_scale, column_scale, bias);
-  *dst = from_float<TO>(MODE == 1 ? to_float(*dst) + value : value);
+__host__ __device__ inline int few_rows_per_block(const FewShape& s) { return (s.rows + s.splits - 1) / s.splits; }
+__host__ __device__ inline int few_recv_row(const FewShape& s) { return s.nb + 4; }  // ints; quads of neighbouring rows in other banks
+__host__ __device__ inline int few_recv_bytes(const FewShape& s) { return s.splits * few_rows_per_block(s) * few_recv_row(s) * 4; }
+// The ring, and what the MMAs of its last slab read beyond the tile's rows; the sums, where they take the ring's place.
+__host__ __device__ inline int few_ring_bytes(const FewShape& s) {
+  const int lanes = s.rows > 128 ? 256 : 128;
+  int bytes = s.stages * few_stage_bytes(s);
+  const int reach = (s.stages - 1) * few_stage_bytes(s) + (s.slabs - 1) * few_w_bytes(s) + lanes * I8_BK;
+  if (reach > bytes) bytes = reach;
+  if (s.splits == 1 && few_recv_bytes(s) > bytes) bytes = (few_recv_bytes(s) + 1023) & ~1023;
+  return bytes;
 }
 
 template <int MODE, typename TO>
@@ -218,180 +235,302 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                      const FewShape shape, const Int8Scales scales, int* error_flag) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  const int stages = shape.stages, nb = shape.nb, splits = shape.splits;
-  const int stage_bytes = few_stage_bytes(nb);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
-  uint64_t* empty = full + stages;
-  uint64_t* acc_full = empty + stages;
+  const int stages = shape.stages, nb = shape.nb, splits = shape.splits, slabs = shape.slabs;
+  const int w_bytes = few_w_bytes(shape), x_bytes = nb * I8_BK, stage_bytes = few_stage_bytes(shape);
+  unsigned char* tail = smem + few_ring_bytes(shape);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tail);
+  uint64_t* empty = full + FEW_MAX_STAGES;
+  uint64_t* acc_full = empty + FEW_MAX_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* recv = reinterpret_cast<int*>(smem + stages * stage_bytes + FEW_TAIL_BYTES);  // [split][row of codes][weight row]
+  float* row_scales = reinterpret_cast<float*>(tail + 512);  // [M]
+  float* column_scales = row_scales + FEW_MAX_ROWS;          // [weight row of the tile]
+  float* biases = column_scales + 256;
+  unsigned char* nowhere = tail + 448;  // 16 bytes
+  // [split][weight row][row of codes]; where K is not split, the ring is free when the sums come
+  int* recv = reinterpret_cast<int*>(splits > 1 ? tail + FEW_TAIL_BYTES : smem);
 
   pdl_trigger();
   if (splits > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = (int)blockIdx.x / splits, split = (int)blockIdx.x - tile * splits;
   const int kb0 = shape.k_iters * split / splits, kb1 = shape.k_iters * (split + 1) / splits;
+  const int groups = shape.rows > 128 ? 2 : 1;
   int tmem_cols = 32;
-  while (tmem_cols < nb) tmem_cols *= 2;
+  while (tmem_cols < groups * nb) tmem_cols *= 2;
+  const int per = few_rows_per_block(shape), recv_row = few_recv_row(shape);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
-    mbar_init(smem_u32(acc_full), 1);
-    *abort_flag = 0;
+  if (warp == 0) {
+    if (lane < stages) { mbar_init(smem_u32(&full[lane]), slabs); mbar_init(smem_u32(&empty[lane]), 1); }
+    if (lane == 0) { mbar_init(smem_u32(acc_full), 1); *abort_flag = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_cols));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  fence_before();
   __syncthreads();
-  fence_after();
-  const uint32_t tmem_base = *tmem_slot;
 
   bool ok = true;
-  if (warp == 0) {
-    if (lane == 0) {
-      // Neighbouring tiles start their walk over K at different slabs: blocks that run at the same time would else ask for the
-      // same lines of the codes, and for addresses a whole weight row apart, at the same moment.
+  auto give_up = [&]() {  // a wait ran out: every role leaves
+    *abort_flag = 1;
+    if (error_flag != nullptr) atomicExch(error_flag, 6);
+  };
+  uint32_t tmem_base = 0;
+  if (warp < FEW_PRODUCERS) {
+    if (elect_one()) {
+      // Slabs are counted from the start of the block's walk: slab u lies in stage u / slabs and is copied by warp u % 4, with the
+      // rows of codes that belong to it.  Neighbouring tiles start their walk over K at different places: blocks that run at the
+      // same time would else ask for the same lines of the codes, and for addresses a whole weight row apart, at the same moment.
       const uint64_t once = policy_evict_first();
-      const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), stage0 = smem_u32(smem);
-      const int count = kb1 - kb0, first = kb0 + tile * 5 % count;
-      auto slab = [&](int i) { const int kb = first + i; return (kb < kb1 ? kb : kb - count) * I8_BK; };
-      const int ahead = min(stages, count);
+      const int count = kb1 - kb0, first = tile * 5 % count;
+      const int units = count * slabs, ahead = min(stages, count) * slabs;
+      const int w_load = shape.rows * I8_BK;
+      struct Walk {
+        int s, i, k;  // stage, slab in the stage, and the stage's place in K
+      };
+      auto begin = [&]() {
+        Walk at;
+        at.s = warp / slabs;
+        at.i = warp % slabs;
+        at.k = first + at.s;
+        while (at.s >= stages) at.s -= stages;
+        while (at.k >= count) at.k -= count;
+        return at;
+      };
+      auto step = [&](Walk& at) {  // four slabs further
+        const int on = FEW_PRODUCERS / slabs;
+        at.s += on;
+        while (at.s >= stages) at.s -= stages;
+        at.k += on;
+        while (at.k >= count) at.k -= count;
+      };
+      auto load_w = [&](const Walk& at) {
+        tma_load_2d(smem_u32(smem) + at.s * stage_bytes + at.i * w_bytes, &map_w, ((kb0 + at.k) * slabs + at.i) * I8_BK,
+                    tile * shape.rows, smem_u32(&full[at.s]), once);
+      };
+      auto load_x = [&](const Walk& at) {
+        tma_load_2d(smem_u32(smem) + at.s * stage_bytes + slabs * w_bytes + at.i * x_bytes, &map_x,
+                    ((kb0 + at.k) * slabs + at.i) * I8_BK, 0, smem_u32(&full[at.s]));
+      };
+      Walk at = begin();
       if (!shape.early) pdl_wait();
-      for (int i = 0; i < ahead; ++i) {
-        mbar_expect_tx(full0 + i * 8, FEW_W_BYTES);
-        tma_load_2d(stage0 + i * stage_bytes, &map_w, slab(i), tile * 128, full0 + i * 8, once);
+      for (int u = warp; u < ahead; u += FEW_PRODUCERS, step(at)) {
+        mbar_expect_tx(smem_u32(&full[at.s]), w_load);
+        load_w(at);
       }
       if (shape.early) pdl_wait();
-      for (int i = 0; i < ahead; ++i) {
-        mbar_arrive_expect_tx(full0 + i * 8, nb * I8_BK);
-        tma_load_2d(stage0 + i * stage_bytes + FEW_W_BYTES, &map_x, slab(i), 0, full0 + i * 8);
+      at = begin();
+      int u = warp;
+      for (; u < ahead; u += FEW_PRODUCERS, step(at)) {
+        mbar_arrive_expect_tx(smem_u32(&full[at.s]), x_bytes);
+        load_x(at);
       }
-      int s = 0;
       uint32_t turn = 0;
-      for (int i = ahead; i < count; ++i) {
-        ok = mbar_wait(empty0 + s * 8, turn, abort_flag);
+      int turn_end = 2 * ahead;  // the slab with which the ring's next turn begins
+      for (; u < units; u += FEW_PRODUCERS, step(at)) {
+        while (u >= turn_end) { turn ^= 1; turn_end += ahead; }
+        ok = mbar_wait(smem_u32(&empty[at.s]), turn, abort_flag);
         if (!ok) break;
-        mbar_arrive_expect_tx(full0 + s * 8, stage_bytes);
-        tma_load_2d(stage0 + s * stage_bytes, &map_w, slab(i), tile * 128, full0 + s * 8, once);
-        tma_load_2d(stage0 + s * stage_bytes + FEW_W_BYTES, &map_x, slab(i), 0, full0 + s * 8);
-        if (++s == stages) { s = 0; turn ^= 1; }
+        mbar_arrive_expect_tx(smem_u32(&full[at.s]), w_load + x_bytes);
+        load_w(at);
+        load_x(at);
       }
+      if (!ok) give_up();
     }
-    if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-  } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = instr_desc_i8(128, nb);
-      int s = 0;
-      uint32_t turn = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {  // in the order in which the producer walks
-        ok = mbar_wait(smem_u32(&full[s]), turn, abort_flag);
-        if (!ok) break;
-        fence_after();
-        const uint64_t desc_w = desc_k_major(smem_u32(smem + s * stage_bytes));
-        const uint64_t desc_x = desc_k_major(smem_u32(smem + s * stage_bytes + FEW_W_BYTES));
-#pragma unroll
-        for (int k = 0; k < I8_BK / I8_UMMA_K; ++k)
-          mma_i8(tmem_base, desc_w + 2 * k, desc_x + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-        commit(smem_u32(&empty[s]));
-        if (++s == stages) { s = 0; turn ^= 1; }
-      }
-      if (ok) commit(smem_u32(acc_full));
-    }
-    if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   } else {
-    if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every block of the cluster runs
-    pdl_wait();  // the scales, and the output, belong to the step
-    const int quarter = warp & 3, r = quarter * 32 + lane, n = tile * 128 + r;
-    const bool inside = n < shape.N;
-    const float column_scale = inside ? scales.columns[n] : 0.f;
-    const float bias = inside && scales.bias != nullptr ? scales.bias[n] : 0.f;
-    const uint32_t tmem_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    ok = mbar_wait(smem_u32(acc_full), 0, abort_flag);
-    if (ok) {
-      fence_after();
-      const int per = few_rows_per_block(splits), owner = r / per;
-      uint32_t remote = 0;
-      if (splits > 1) {
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(recv)), "r"(owner));
-        remote += (uint32_t)((split * nb * per + r - owner * per) * 4);
-      }
-      for (int c = 0; c < shape.M; c += 16) {
-        uint32_t v[16];
-        tmem_ld16(v, tmem_row + c);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (c + j >= shape.M) break;
-          if (splits > 1)
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote + (uint32_t)((c + j) * per * 4)), "r"(v[j]) : "memory");
-          else if (inside)
-            few_store<MODE>(out + (size_t)(c + j) * shape.ldo + n, (int)v[j], scales.rows[c + j], column_scale, bias);
-        }
-      }
-      fence_before();
+    if (warp == FEW_PRODUCERS) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_cols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    fence_before();
+    asm volatile("bar.sync 2, 160;" ::: "memory");  // the MMA warp and the finishing warps
+    fence_after();
+    tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   }
-  if (!ok && lane == 0) { *abort_flag = 1; if (error_flag != nullptr) atomicExch(error_flag, 6); }
-
-  if (splits > 1) {
-    // Every thread of every block of the cluster comes here, also after a wait that ran out.  After the meeting nothing
-    // touches another block's memory, so a block may leave when it is done.
-    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-    if (warp >= 2 && !*abort_flag) {
-      const int per = few_rows_per_block(splits), row_lo = split * per;
-      const int n_lo = tile * 128 + row_lo, here = max(0, min(min(per, 128 - row_lo), shape.N - n_lo));
-      for (int idx = (int)threadIdx.x - 64; idx < here * shape.M; idx += 128) {
-        const int m = idx / here, local = idx - m * here, n = n_lo + local;
-        int sum = 0;
-        for (int sp = 0; sp < splits; ++sp) sum += recv[(sp * nb + m) * per + local];
-        few_store<MODE>(out + (size_t)m * shape.ldo + n, sum, scales.rows[m], scales.columns[n],
-                        scales.bias != nullptr ? scales.bias[n] : 0.f);
+  if (warp == FEW_PRODUCERS && elect_one()) {
+    const uint32_t idesc = instr_desc_i8(128, nb);
+    int s = 0;
+    uint32_t turn = 0;
+    auto slab = [&](uint64_t desc_w, uint64_t desc_x, auto adds) {  // `adds`: whether to the sums so far
+#pragma unroll
+      for (int k = 0; k < I8_BK / I8_UMMA_K; ++k) {  // 32 bytes further along K inside the swizzle atom
+        mma_i8(tmem_base, desc_w + 2 * k, desc_x + 2 * k, idesc, decltype(adds)::value || k > 0);
+        if (groups == 2) mma_i8(tmem_base + nb, desc_w + 2 * k + (128 * I8_BK >> 4), desc_x + 2 * k, idesc, decltype(adds)::value || k > 0);
+      }
+    };
+    for (int kb = kb0; kb < kb1; ++kb) {  // in the order in which the producers walk
+      ok = mbar_wait(smem_u32(&full[s]), turn, abort_flag);
+      if (!ok) break;
+      fence_after();
+      const uint64_t desc_w = desc_k_major(smem_u32(smem) + s * stage_bytes);
+      const uint64_t desc_x = desc_k_major(smem_u32(smem) + s * stage_bytes + slabs * w_bytes);
+      if (kb == kb0) slab(desc_w, desc_x, std::false_type());
+      else slab(desc_w, desc_x, std::true_type());
+      for (int i = 1; i < slabs; ++i) slab(desc_w + (i * w_bytes >> 4), desc_x + (i * x_bytes >> 4), std::true_type());
+      commit(smem_u32(&empty[s]));
+      if (++s == stages) { s = 0; turn ^= 1; }
+    }
+    if (ok) commit(smem_u32(acc_full));
+    else give_up();
+  }
+  if (warp > FEW_PRODUCERS) {
+    const int tid = (int)threadIdx.x - 32 * (FEW_PRODUCERS + 1);
+    pdl_wait();  // the scales, and the output, belong to the step
+    for (int i = tid; i < nb; i += 128) row_scales[i] = i < shape.M ? scales.rows[i] : 0.f;
+    for (int i = tid; i < shape.rows; i += 128) {
+      const int n = min(tile * shape.rows + i, shape.N - 1);
+      column_scales[i] = scales.columns[n];
+      biases[i] = scales.bias != nullptr ? scales.bias[n] : 0.f;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  }
+  const int row_lo = split * per, n_lo = tile * shape.rows + row_lo;
+  const int here = max(0, min(min(per, shape.rows - row_lo), shape.N - n_lo)), quads = (shape.M + 3) / 4;
+#pragma unroll 1
+  for (int pass = warp > FEW_PRODUCERS ? 0 : 1; pass < 2; ++pass) {
+    if (pass == 1) {
+      if (splits > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every block of the cluster runs
+      if (warp > FEW_PRODUCERS) {
+        const int quarter = warp & 3;
+        ok = mbar_wait(smem_u32(acc_full), 0, abort_flag);
+        if (!ok && lane == 0) give_up();
+        fence_after();
+        for (int g = 0; ok && g < groups; ++g) {
+          const int r = g * 128 + quarter * 32 + lane, owner = min(r, shape.rows - 1) / per;
+          uint32_t to;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(recv)), "r"(owner));
+          to += (uint32_t)((split * per + r - owner * per) * recv_row * 4);
+#pragma unroll 1
+          for (int c = 0; c < shape.M; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(v, tmem_base + ((uint32_t)(quarter * 32) << 16) + g * nb + c);
+            tmem_wait_ld();
+            if (r < shape.rows) {
+#pragma unroll
+              for (int j = 0; j < 16; j += 4)
+                asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)((c + j) * 4)), "r"(v[j]),
+                             "r"(v[j + 1]), "r"(v[j + 2]), "r"(v[j + 3]) : "memory");
+            }
+          }
+        }
+        fence_before();
+      }
+      // Every thread of the cluster comes here, also after a wait that ran out.  After this meeting nothing touches another
+      // block's memory, so a block may leave when it is done.
+      if (splits > 1) asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+      else __syncthreads();
+      if (*abort_flag) break;
+    }
+    const int begin = pass == 1 ? (int)threadIdx.x : 0, end = pass == 1 ? here * quads : 1, wide = max(here, 1);
+#pragma unroll 1
+    for (int idx = begin; idx < end; idx += FEW_THREADS) {
+      const int quad = idx / wide, local = idx - quad * wide;
+      int sums[4] = {0, 0, 0, 0};
+#pragma unroll 1
+      for (int sp = 0; sp < splits; ++sp) {
+        const int4 part = *reinterpret_cast<const int4*>(recv + (sp * per + local) * recv_row + quad * 4);
+        sums[0] += part.x; sums[1] += part.y; sums[2] += part.z; sums[3] += part.w;
+      }
+      const float4 by_row = *reinterpret_cast<const float4*>(row_scales + quad * 4);
+      const float by_column = column_scales[row_lo + local], bias = biases[row_lo + local];
+      const float factors[4] = {by_row.x, by_row.y, by_row.z, by_row.w};
+      // rows beyond M, and all rows of the first walk, go nowhere; what is added into is asked for before the first store,
+      // which might be to the same memory
+      TO* dst[4];
+      float old[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = quad * 4 + e;
+        dst[e] = pass == 1 && m < shape.M ? out + (size_t)m * shape.ldo + n_lo + local : reinterpret_cast<TO*>(nowhere);
+        old[e] = MODE == 1 ? to_float(*dst[e]) : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float value = fmaf(__int2float_rn(sums[e]) * factors[e], by_column, bias);
+        *dst[e] = from_float<TO>(MODE == 1 ? old[e] + value : value);
       }
     }
   }
   __syncthreads();
-  if (warp == 1) {
+  if (warp == FEW_PRODUCERS) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols));
   }
 }
 
-static int few_shared_bytes(int nb, int splits, int stages) {
-  const int recv = splits > 1 ? splits * nb * few_rows_per_block(splits) * 4 : 0;
-  return stages * few_stage_bytes(nb) + FEW_TAIL_BYTES + recv + 1024;
+static int few_shared_bytes(const FewShape& s) {
+  return few_ring_bytes(s) + FEW_TAIL_BYTES + (s.splits > 1 ? few_recv_bytes(s) : 0) + 1024;
 }
 
-static int plan_few(FewShape& shape, int tiles, int sm_count) {
-  const int two = 113 * 1024, most = 227 * 1024;
-  int splits = 1;
-  while (splits < FEW_MAX_SPLITS && tiles * (splits + 1) <= 2 * sm_count && shape.k_iters >= 4 * (splits + 1)) ++splits;
-  shape.splits = splits;
-  const int share = (shape.k_iters + splits - 1) / splits;
-  for (int limit : {two, most}) {
-    shape.stages = 12;
-    while (shape.stages > 1 && few_shared_bytes(shape.nb, splits, shape.stages) > limit) --shape.stages;
-    if (shape.stages >= 3) break;
+// The tile, the parts of K and the ring of a product, from what was measured on a B200 (148 multiprocessors).
+//
+// Up to 128 weight rows a multiprocessor, one block each: the time is the longer of W from memory (6.3 TB/s in all, 110 GB/s
+// into one multiprocessor) and a block's walk over its slabs (0.15 us each, or their bytes at 110 GB/s), a third of the
+// shorter, and what it takes to begin and end: 2 us, and where the parts of a tile meet 0.8 us more and 0.4 us for each
+// 1,000 sums that a block sends.  Clusters of 3 and 4 do not fill the device (45 and 33 are held; many fewer of 3 at once in
+// practice).  Microseconds, chosen against the next best number of parts: 8 rows of 4,096 outputs, 4,096 inputs 5.9 (4 parts; 2: 6.0,
+// 1: 7.8); 6,144, 4,096 7.1 (2; 4: 7.5); 4,096, 14,336 12.4 (4; 3: 12.8); 64 of 2,048, 2,048 4.8 (2; 4: 5.2).
+//
+// More weight rows than that: K is not split.  Two blocks a multiprocessor with a ring of four slabs each, if their
+// tiles make one round of it or even tiles of 256 rows do not (8 rows of 28,672 outputs, 4,096 inputs 19.1 against 19.8 with one
+// block, 64 rows 22.5 against 24.8); else one block with tiles of up to 256 rows (128 rows 30.7).
+constexpr int FEW_SHARED_ONE = 227 * 1024, FEW_SHARED_TWO = 113 * 1024;
+
+static void plan_few(FewShape& s, int K, int sm_count) {
+  const int slabs = (K + I8_BK - 1) / I8_BK;
+  auto even_rows = [&](int blocks) { return ((s.N + blocks - 1) / blocks + 7) / 8 * 8; };
+  int limit = FEW_SHARED_ONE;
+  if (even_rows(sm_count) <= 128) {
+    double best = 0;
+    s.splits = 0;
+    for (int splits = 1; splits <= 4 && (splits == 1 || slabs >= 4 * splits); ++splits) {
+      const int blocks = splits <= 2 ? sm_count : splits == 3 ? sm_count * 4 / 5 : sm_count * 8 / 9;
+      if (blocks < splits) break;
+      const int even = even_rows(blocks / splits);
+      for (int rows : {32, 64, 96, 128, even}) {
+        if (rows > 256 || rows < even) continue;
+        const int used = (s.N + rows - 1) / rows * splits;
+        const double rate = used * 0.11e6 < 6.3e6 ? used * 0.11e6 : 6.3e6, slab_us = (rows + s.M) * 128 / 110e3;
+        const double memory_us = (double)s.N * K / rate;
+        const double walk_us = (slabs + splits - 1) / splits * (slab_us > 0.15 ? slab_us : 0.15);
+        const double longer = memory_us > walk_us ? memory_us : walk_us;
+        const double cost = longer + 0.3 * (memory_us + walk_us - longer) + (splits > 1 ? 0.8 + 0.4e-3 * rows * s.M : 0.0);
+        if (s.splits == 0 || cost < best) { best = cost; s.splits = splits; s.rows = rows; }
+      }
+    }
+  } else {
+    const int two_most = 220 - s.nb;  // weight rows that leave room for four slabs
+    const int two_rounds = (s.N + 2 * sm_count * two_most - 1) / (2 * sm_count * two_most);
+    const int one_rounds = (s.N + sm_count * 256 - 1) / (sm_count * 256);
+    const bool two = two_rounds == 1 || one_rounds > 1;
+    s.splits = 1;
+    s.rows = two ? even_rows(2 * sm_count * two_rounds) : even_rows(sm_count);
+    if (two) limit = FEW_SHARED_TWO;
   }
-  if (shape.stages > share) shape.stages = share;
-  return few_shared_bytes(shape.nb, splits, shape.stages);
+  // slabs a stage: as many as leave a ring of three stages
+  for (s.slabs = 4; s.slabs > 1; s.slabs /= 2) {
+    s.stages = 3;
+    if (few_shared_bytes(s) <= limit) break;
+  }
+  s.k_iters = (slabs + s.slabs - 1) / s.slabs;
+  const int share = (s.k_iters + s.splits - 1) / s.splits;
+  for (;;) {
+    s.stages = FEW_MAX_STAGES;
+    while (s.stages > 1 && few_shared_bytes(s) > limit) --s.stages;
+    // the producers, which take every fourth slab each, need a ring of four slabs if it turns
+    if (s.stages * s.slabs >= FEW_PRODUCERS || s.stages >= share || limit == FEW_SHARED_ONE) break;
+    limit = FEW_SHARED_ONE;
+  }
+  if (s.stages > share) s.stages = share;
 }
 
 template <int MODE, typename TO>
-int launch_gemm_int8_few(void* out, const CUtensorMap& map_w, const CUtensorMap& map_x, FewShape shape, const Int8Scales& scales,
-                         int sm_count, int* error_flag, cudaStream_t stream) {
+int launch_gemm_int8_few(void* out, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewShape& shape, const Int8Scales& scales,
+                         int* error_flag, cudaStream_t stream) {
   constexpr auto kernel = gemm_int8_few_kernel<MODE, TO>;
-  const cudaError_t err = allow_shared_memory_once<kernel>(227 * 1024);
+  const cudaError_t err = allow_shared_memory_once<kernel>(FEW_SHARED_ONE);
   if (err != cudaSuccess) return (int)err;
-  const int tiles = (shape.N + 127) / 128;
-  const int smem = plan_few(shape, tiles, sm_count);
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)tiles * shape.splits);
+  config.gridDim = dim3((unsigned)((shape.N + shape.rows - 1) / shape.rows) * shape.splits);
   config.blockDim = dim3(FEW_THREADS);
-  config.dynamicSmemBytes = smem;
+  config.dynamicSmemBytes = few_shared_bytes(shape);
   config.stream = stream;
   cudaLaunchAttribute attrs[2];
   int n_attrs = 0;
@@ -425,12 +564,17 @@ XRT_EXPORT int xrt_gemm_int8(void* out, const void* codes, const float* scales, 
   CUtensorMap map_x, map_w;
   const xrt::Int8Scales factors{scales, w_scales, bias};
   if (M <= xrt::FEW_MAX_ROWS) {
-    const xrt::FewShape shape{M, N, ldo, (M + 15) / 16 * 16, 1, 1, (K + xrt::I8_BK - 1) / xrt::I8_BK, constant_weight};
-    if (!xrt::sm100::make_map_int8_2d(&map_x, codes, M, K, ldx, shape.nb) || !xrt::sm100::make_map_int8_2d(&map_w, w, N, K, ldw, 128))
+    xrt::FewShape shape = {};
+    shape.M = M; shape.N = N; shape.ldo = ldo;
+    shape.nb = (M + 15) / 16 * 16;
+    shape.early = constant_weight;
+    xrt::plan_few(shape, K, sm_count);
+    if (!xrt::sm100::make_map_int8_2d(&map_x, codes, M, K, ldx, shape.nb) ||
+        !xrt::sm100::make_map_int8_2d(&map_w, w, N, K, ldw, shape.rows))
       return XRT_ERR_UNSUPPORTED;
-    if (mode == 1) return xrt::launch_gemm_int8_few<1, float>(out, map_w, map_x, shape, factors, sm_count, error_flag, stream);
+    if (mode == 1) return xrt::launch_gemm_int8_few<1, float>(out, map_w, map_x, shape, factors, error_flag, stream);
     XRT_DISPATCH_DTYPE(out_dtype, TO, {
-      return xrt::launch_gemm_int8_few<0, TO>(out, map_w, map_x, shape, factors, sm_count, error_flag, stream);
+      return xrt::launch_gemm_int8_few<0, TO>(out, map_w, map_x, shape, factors, error_flag, stream);
     });
   }
   if (!xrt::sm100::make_map_int8_2d(&map_x, codes, M, K, ldx, 128) || !xrt::sm100::make_map_int8_2d(&map_w, w, N, K, ldw, 128))

@@ -1703,38 +1703,49 @@ def int8_rows(rows: int, width: int, device) -> torch.Tensor:
     return torch.empty((rows, -(-width // 16) * 16), dtype=torch.int8, device=device)[:, :width]
 
 
-def _launch_on(what: str, tensors, call) -> None:
-    """``call(stream)`` on the one device that all of ``tensors`` (None: not given) lie on, whichever is current."""
-    device = tensors[0].device
+# A launch of a few microseconds should not wait for its checks: the raw handle of a device's current stream and the current
+# device's number cost a tenth of a microsecond each, ``torch.cuda.current_stream`` two.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _run_int8(what: str, tensors, function: str, args) -> None:
+    """Calls a launcher on the one device that all of ``tensors`` (None: not given) lie on, whichever is current, and on
+    that device's current stream."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != device):
+        if t is not None and (t.get_device() != index or index < 0):
             raise KernelError(f"{what}: all tensors must be on one CUDA device")
-    lib = _kernels()
-    if device.index == torch.cuda.current_device():
-        _check(call(lib, torch.cuda.current_stream(device).cuda_stream), what)
+    launcher = getattr(_lib or library(), function)
+    if index == torch.cuda.current_device():
+        _check(launcher(*args, _raw_stream(index)), what)
     else:
-        with torch.cuda.device(device):
-            _check(call(lib, torch.cuda.current_stream(device).cuda_stream), what)
+        with torch.cuda.device(index):
+            _check(launcher(*args, _raw_stream(index)), what)
 
 
-def _error_flag_pointer(device) -> int:
-    """The device's error flag for a launch; 0 (the kernel reports nothing) where it would have to be made inside a capture."""
-    if device.index not in _error_flags and torch.cuda.is_current_stream_capturing():
-        return 0
-    return error_flag(device).data_ptr()
+def _error_flag_pointer(index: int) -> int:
+    """A device's error flag for a launch; 0 (the kernel reports nothing) where it would have to be made inside a capture."""
+    flag = _error_flags.get(index)
+    if flag is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        flag = error_flag(torch.device("cuda", index))
+    return flag.data_ptr()
 
 
 def _codes(t, name: str, what: str, rows: int, width: int) -> int:
     """The distance of the rows of an int8 tensor [rows, width] in bytes."""
-    if t.dtype != torch.int8 or tuple(t.shape) != (rows, width):
+    if t.dtype != torch.int8 or t.shape != (rows, width):
         raise KernelError(f"{what}: {name} must be int8 [{rows}, {width}], not {t.dtype} {tuple(t.shape)}")
-    if (width > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < width):
+    distance, step = t.stride()
+    if (width > 1 and step != 1) or (rows > 1 and distance < width):
         raise KernelError(f"{what}: the rows of {name} must be contiguous")
-    return t.stride(0) if rows > 1 else -(-width // 16) * 16
+    return distance if rows > 1 else -(-width // 16) * 16
 
 
 def _vector(t, name: str, what: str, size: int) -> int:
-    if t.dtype != torch.float32 or tuple(t.shape) != (size,) or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.shape != (size,) or not t.is_contiguous():
         raise KernelError(f"{what}: {name} must be float32 [{size}] without gaps, not {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -1750,7 +1761,7 @@ def quantize_rows(codes, scales, x) -> None:
     n, width = x.shape
     ld = _codes(codes, "codes", what, n, width)
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), n, width, ld, _code(x.dtype))
-    _launch_on(what, (x, codes, scales), lambda lib, stream: lib.xrt_quantize_rows(*args, stream))
+    _run_int8(what, (x, codes, scales), "xrt_quantize_rows", args)
 
 
 def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
@@ -1767,7 +1778,7 @@ def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
     options = gate.options(width)
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), n, width, ld, _code(gate_up.dtype),
             code, options)
-    _launch_on(what, (gate_up, codes, scales, gate.bias), lambda lib, stream: lib.xrt_swiglu_int8(*args, stream))
+    _run_int8(what, (gate_up, codes, scales, gate.bias), "xrt_swiglu_int8", args)
 
 
 def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None) -> None:
@@ -1789,7 +1800,7 @@ def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None) -> No
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),
             _ptr(out, "out", torch.float32), _ptr(weight, "weight"), n, width, ld, float(eps),
             0 if add is None else _code(add.dtype), _code(weight.dtype))
-    _launch_on(what, (x, codes, scales, weight, add, out), lambda lib, stream: lib.xrt_rmsnorm_int8(*args, stream))
+    _run_int8(what, (x, codes, scales, weight, add, out), "xrt_rmsnorm_int8", args)
 
 
 def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = False, bias=None,
@@ -1803,19 +1814,23 @@ def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = Fals
     what = "gemm_int8"
     if codes.dim() != 2 or weight.dim() != 2 or codes.shape[1] != weight.shape[1]:
         raise KernelError(f"{what}: shapes do not fit: codes {tuple(codes.shape)}, weight {tuple(weight.shape)}")
-    (m, k), n = codes.shape, weight.shape[0]
+    m, k = codes.shape
+    n = weight.shape[0]
     if k > INT8_MAX_INPUTS:
         raise KernelError(f"{what}: sums over {k} inputs can pass 32 bits; at most {INT8_MAX_INPUTS} are taken")
     ldx, ldw = _codes(codes, "codes", what, m, k), _codes(weight, "weight", what, n, k)
-    for name, t, ld in (("codes", codes, ldx), ("weight", weight, ldw)):
-        if ld % 16 or t.data_ptr() % 16:
-            raise KernelError(f"{what}: the rows of {name} must begin every so many 16 bytes (see int8_rows)")
-    if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
-        raise KernelError(f"{what}: out must be [{m}, {n}] with contiguous rows")
+    if (ldx | ldw | codes.data_ptr() | weight.data_ptr()) % 16:
+        name = "codes" if (ldx | codes.data_ptr()) % 16 else "weight"
+        raise KernelError(f"{what}: the rows of {name} must begin every so many 16 bytes (see int8_rows)")
+    if out.shape != (m, n):
+        raise KernelError(f"{what}: out must be [{m}, {n}], not {tuple(out.shape)}")
+    out_distance, step = out.stride()
+    if (n > 1 and step != 1) or (m > 1 and out_distance < n):
+        raise KernelError(f"{what}: the rows of out must be contiguous")
     if accumulate and out.dtype != torch.float32:
         raise KernelError(f"{what}: only a float32 out is added into")
     args = (out.data_ptr(), codes.data_ptr(), _vector(scales, "scales", what, m), weight.data_ptr(),
             _vector(weight_scales, "weight_scales", what, n), 0 if bias is None else _vector(bias, "bias", what, n), m, n, k,
-            ldx, ldw, out.stride(0) if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0)
-    _launch_on(what, (out, codes, scales, weight, weight_scales, bias),
-               lambda lib, stream: lib.xrt_gemm_int8(*args, _error_flag_pointer(out.device), stream))
+            ldx, ldw, out_distance if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0,
+            _error_flag_pointer(out.get_device()) if out.is_cuda else 0)
+    _run_int8(what, (out, codes, scales, weight, weight_scales, bias), "xrt_gemm_int8", args)

@@ -17,6 +17,15 @@ constexpr long long SPIN_LIMIT = 1ll << 24;  // polls of a barrier before a wait
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// One lane of a warp whose lanes are all here.  The compiler knows it for one lane, and so that the operands of what it issues are
+// the same for the warp, as tcgen05.mma and the copies want them; behind `lane == 0` it does not, and every issue pays for
+// that (measured, clocks from one tcgen05.mma of 128 x 16 to the next: 186 behind `lane == 0`, 39 behind this).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(chosen));
+  return chosen != 0;
+}
+
 __device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }

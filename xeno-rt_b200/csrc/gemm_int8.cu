@@ -3,13 +3,17 @@
 // order, and are rounded to 32-bit floating point once, before the scales.  K is bounded by the caller's check, so that
 // 128 * 128 * K stays below 2^31.
 //
-// A persistent block, one a multiprocessor, walks output tiles of 128 x 256.  Six warps a block:
-//   warp 0     producer: for each 128-wide slab of K, TMA loads of the block's 128 rows of codes and 256 rows of W into the next
-//              free stage of a ring; what a tile has beyond M, N or K arrives as zeros.
-//   warp 1     allocates TMEM (two accumulators of 128 lanes x 256 columns) and issues the MMAs: four a stage, each 32 bytes
-//              of K.
-//   warps 2-5  epilogue: each warp reads its 32 TMEM lanes (rows), 32 columns at a time, applies the scales, turns the
-//              patch around in shared memory and stores 16 bytes a lane, while the MMA warp fills the other accumulator.
+// Many rows: a persistent block, or a pair of blocks as one (cta_group::2, Int8Shape), one block a multiprocessor, walks output
+// tiles of 128 (a pair: 256) rows and BN columns.  Seven warps a block:
+//   warps 0, 1  producers, one of the block's 128 rows of codes, one of its rows of W (in a pair half of the tile's): for each
+//               128-wide slab of K a TMA load into the next free stage of a ring; what a tile has beyond M, N or K
+//               arrives as zeros.
+//   warp 2      owns TMEM (two accumulators of 128 lanes x BN columns) and issues the MMAs (in a pair the first block's does,
+//               for both): four a stage, each 32 bytes of K.
+//   warps 3-6   epilogue: each warp reads its 32 TMEM lanes (rows), 32 columns at a time, applies the scales and writes
+//               patches of 32 rows x 128 bytes to shared memory, which a TMA store takes (or a TMA reduction adds into the
+//               output), while the MMA warp fills the other accumulator.  Outputs whose rows do not begin every 16
+//               bytes are stored by the warp, a row of 32 columns at a time.
 // Every wait on an mbarrier is bounded.  A wait that runs out raises the error flag and an abort flag in shared memory; all
 // roles leave their loops, the block frees its TMEM and returns.
 #include <type_traits>
@@ -20,12 +24,18 @@ namespace xrt {
 
 using namespace sm100;
 
-constexpr int I8_BM = 128, I8_BN = 256, I8_BK = 128, I8_UMMA_K = 32;
-constexpr int I8_A_BYTES = I8_BM * I8_BK, I8_B_BYTES = I8_BN * I8_BK;
-constexpr int I8_STAGES = 4, I8_STAGE_BYTES = I8_A_BYTES + I8_B_BYTES;
-constexpr int I8_THREADS = 192;
-constexpr int I8_STAGING_BYTES = 4 * 32 * 33 * 4;
-constexpr int I8_SMEM = I8_STAGES * I8_STAGE_BYTES + I8_STAGING_BYTES + 256 + 1024;
+constexpr int I8_BM = 128, I8_BK = 128, I8_UMMA_K = 32;
+constexpr int I8_THREADS = 32 * 7;
+template <bool PAIR, int BN> struct Int8Shape {
+  static constexpr int A_BYTES = I8_BM * I8_BK;
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // of the W tile, in one block
+  static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * I8_BK;
+  static constexpr int STAGES = 196608 / STAGE_BYTES;
+  static constexpr int PATCH_BYTES = 5120;             // an epilogue warp's: 32 x 128 bytes, or 32 rows of 33 floats
+  static constexpr int STAGING_BYTES = 4 * PATCH_BYTES;
+  static constexpr int FACTOR_BYTES = 2 * 2 * BN * 4;  // scales and biases of a tile's columns, one set an accumulator
+  static constexpr int SMEM = STAGES * STAGE_BYTES + STAGING_BYTES + FACTOR_BYTES + 512 + 1024;
+};
 
 // What the sums are multiplied by and what is added.
 struct Int8Scales {
@@ -34,153 +44,339 @@ struct Int8Scales {
   const float* bias;     // [N] or null
 };
 
+// Where a tile lies.  Tiles that run at the same time should share operands in the L2: the walk goes down 4,096 rows of codes,
+// then to the next column of tiles, and only after the last column to the next such group of rows.
+template <int TILE_ROWS>
+__device__ __forceinline__ void int8_tile_place(int tile, int tiles_m, int tiles_n, int& m_blk, int& n_blk) {
+  constexpr int GROUP = 4096 / TILE_ROWS;
+  const int per_group = GROUP * tiles_n;
+  const int group = tile / per_group, in_group = tile - group * per_group;
+  const int rows = min(GROUP, tiles_m - group * GROUP);
+  n_blk = in_group / rows;
+  m_blk = group * GROUP + (in_group - n_blk * rows);
+}
+
+// 16 bytes of a patch's row: four float32 or eight bfloat16 from value `at` on.
+template <typename TO>
+__device__ __forceinline__ uint4 int8_unit(const float (&v)[32], int at);
+template <>
+__device__ __forceinline__ uint4 int8_unit<float>(const float (&v)[32], int at) {
+  return make_uint4(__float_as_uint(v[at]), __float_as_uint(v[at + 1]), __float_as_uint(v[at + 2]), __float_as_uint(v[at + 3]));
+}
+template <>
+__device__ __forceinline__ uint4 int8_unit<__nv_bfloat16>(const float (&v)[32], int at) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(v[at + 2 * i], v[at + 2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&two);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // MODE 0: store, 1: add into float out.
-template <int MODE, typename TO>
+template <int MODE, bool PAIR, int BN, typename TO>
 __global__ void __launch_bounds__(I8_THREADS, 1)
-gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, TO* __restrict__ out,
-                 int M, int N, int K, int ldo, const Int8Scales scales, int* __restrict__ error_flag) {
+gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                 const __grid_constant__ CUtensorMap map_out, TO* out, int by_tma, int M, int N, int K, int ldo,
+                 const Int8Scales scales, int* error_flag) {
+  using Shape = Int8Shape<PAIR, BN>;
+  constexpr int STAGES = Shape::STAGES, TILE_ROWS = (PAIR ? 2 : 1) * I8_BM;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* a_stages = smem;
-  unsigned char* b_stages = smem + I8_STAGES * I8_A_BYTES;
-  float* staging = reinterpret_cast<float*>(smem + I8_STAGES * I8_STAGE_BYTES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + I8_STAGES * I8_STAGE_BYTES + I8_STAGING_BYTES);
-  uint64_t* empty = full + I8_STAGES;
-  uint64_t* acc_full = empty + I8_STAGES;
+  unsigned char* b_stages = smem + STAGES * Shape::A_BYTES;
+  unsigned char* staging = smem + STAGES * Shape::STAGE_BYTES;
+  float* factors = reinterpret_cast<float*>(staging + Shape::STAGING_BYTES);  // [accumulator][scales, biases][column]
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + Shape::STAGING_BYTES + Shape::FACTOR_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles_m = (M + I8_BM - 1) / I8_BM, tiles_n = (N + I8_BN - 1) / I8_BN;
+  const int tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS, tiles_n = (N + BN - 1) / BN;
   const int n_tiles = tiles_m * tiles_n;
   const int k_iters = (K + I8_BK - 1) / I8_BK;
+  const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // the block's place in its pair
+  const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < I8_STAGES; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&acc_full[a]), 1); mbar_init(smem_u32(&acc_empty[a]), 128); }
+    // a stage is full when the producers (two, in a pair two of each block) have announced their bytes and those are there
+    for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full[s]), 2); mbar_init(smem_u32(&empty[s]), 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&acc_full[a]), 1); mbar_init(smem_u32(&acc_empty[a]), PAIR ? 256 : 128); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if (warp == 2) {
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // the other block's barriers stand before anything arrives on them
   fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
   bool ok = true;
-  if (warp == 0) {
+  auto give_up = [&]() {  // a wait ran out: every role leaves
+    *abort_flag = 1;
+    if (error_flag != nullptr) atomicExch(error_flag, 6);
+  };
+  if (warp < 2) {
     if (elect_one()) {
-      int it = 0;
-      for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
-        const int m0 = tile % tiles_m * I8_BM, n0 = tile / tiles_m * I8_BN;
-        for (int kb = 0; kb < k_iters; ++kb, ++it) {
-          const int s = it % I8_STAGES;
-          ok = mbar_wait(smem_u32(&empty[s]), ((it / I8_STAGES) & 1) ^ 1, abort_flag);
+      const bool codes = warp == 0;
+      const CUtensorMap* map = codes ? &map_x : &map_w;
+      asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+      pdl_wait();
+      const uint32_t stages = smem_u32(codes ? a_stages : b_stages), bytes = codes ? Shape::A_BYTES : Shape::B_ROWS * I8_BK;
+      int s = 0;
+      uint32_t turn = 1;
+      for (int tile = unit; tile < n_tiles && ok; tile += units) {
+        int m_blk, n_blk;
+        int8_tile_place<TILE_ROWS>(tile, tiles_m, tiles_n, m_blk, n_blk);
+        const int row0 = codes ? m_blk * TILE_ROWS + rank * I8_BM : n_blk * BN + rank * Shape::B_ROWS;
+        for (int kb = 0; kb < k_iters; ++kb) {
+          ok = mbar_wait(smem_u32(&empty[s]), turn, abort_flag);
           if (!ok) break;
-          const uint32_t bar = smem_u32(&full[s]), b_dst = smem_u32(b_stages + s * I8_B_BYTES);
-          mbar_arrive_expect_tx(bar, I8_STAGE_BYTES);
-          tma_load_2d(smem_u32(a_stages + s * I8_A_BYTES), &map_x, kb * I8_BK, m0, bar);
-          tma_load_2d(b_dst, &map_w, kb * I8_BK, n0, bar);
-          tma_load_2d(b_dst + I8_B_BYTES / 2, &map_w, kb * I8_BK, n0 + 128, bar);
+          if (PAIR) {
+            // both blocks' copies complete on the first block's barrier, which alone the MMAs wait for; the bytes of both are
+            // announced there (a copy of the second block may complete before that: the phase cannot end without the
+            // arrivals, and the second block reuses a stage only after the MMAs have released it)
+            if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full[s]), 2 * bytes);
+            tma_load_2d_pair(stages + s * bytes, map, kb * I8_BK, row0, first_block_address(smem_u32(&full[s])));
+          } else {
+            mbar_arrive_expect_tx(smem_u32(&full[s]), bytes);
+            tma_load_2d(stages + s * bytes, map, kb * I8_BK, row0, smem_u32(&full[s]));
+          }
+          if (++s == STAGES) { s = 0; turn ^= 1; }
         }
       }
+      // a block of a pair leaves only when the other's MMAs have let go of its last stages
+      for (int j = 0; PAIR && ok && j < STAGES; ++j) {
+        ok = mbar_wait(smem_u32(&empty[s]), turn, abort_flag);
+        if (++s == STAGES) { s = 0; turn ^= 1; }
+      }
+      if (!ok) give_up();
     }
-  } else if (warp == 1) {
-    if (elect_one()) {
-      constexpr uint32_t idesc = instr_desc_i8(I8_BM, I8_BN);
-      int it = 0, tile_i = 0;
-      for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x, ++tile_i) {
-        const int a = tile_i & 1;
-        ok = mbar_wait(smem_u32(&acc_empty[a]), ((tile_i >> 1) & 1) ^ 1, abort_flag);
+  } else if (warp == 2) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = instr_desc_i8(TILE_ROWS, BN);
+      auto slab = [&](uint32_t d, int s, auto adds) {  // `adds`: whether to the sums so far
+        const uint64_t desc_a = desc_k_major(smem_u32(a_stages + s * Shape::A_BYTES));
+        const uint64_t desc_b = desc_k_major(smem_u32(b_stages + s * Shape::B_ROWS * I8_BK));
+#pragma unroll
+        for (int k = 0; k < I8_BK / I8_UMMA_K; ++k) {  // 32 bytes further along K inside the swizzle atom
+          if (PAIR) mma_i8_pair(d, desc_a + 2 * k, desc_b + 2 * k, idesc, decltype(adds)::value || k > 0);
+          else mma_i8(d, desc_a + 2 * k, desc_b + 2 * k, idesc, decltype(adds)::value || k > 0);
+        }
+        if (PAIR) commit_pair(smem_u32(&empty[s]));
+        else commit(smem_u32(&empty[s]));
+      };
+      int s = 0, a = 0;
+      uint32_t turn = 0, acc_turn = 1;
+      for (int tile = unit; tile < n_tiles && ok; tile += units) {
+        ok = mbar_wait(smem_u32(&acc_empty[a]), acc_turn, abort_flag);
         if (!ok) break;
         fence_after();
-        for (int kb = 0; kb < k_iters; ++kb, ++it) {
-          const int s = it % I8_STAGES;
-          ok = mbar_wait(smem_u32(&full[s]), (it / I8_STAGES) & 1, abort_flag);
+        for (int kb = 0; kb < k_iters; ++kb) {
+          ok = mbar_wait(smem_u32(&full[s]), turn, abort_flag);
           if (!ok) break;
           fence_after();
-          const uint64_t desc_a = desc_k_major(smem_u32(a_stages + s * I8_A_BYTES));
-          const uint64_t desc_b = desc_k_major(smem_u32(b_stages + s * I8_B_BYTES));
-#pragma unroll
-          for (int k = 0; k < I8_BK / I8_UMMA_K; ++k)  // 32 bytes further along K inside the swizzle atom
-            mma_i8(tmem_base + a * I8_BN, desc_a + 2 * k, desc_b + 2 * k, idesc, (kb | k) != 0);
-          commit(smem_u32(&empty[s]));
+          if (kb == 0) slab(tmem_base + a * BN, s, std::false_type());
+          else slab(tmem_base + a * BN, s, std::true_type());
+          if (++s == STAGES) { s = 0; turn ^= 1; }
         }
-        if (ok) commit(smem_u32(&acc_full[a]));
+        if (!ok) break;
+        if (PAIR) commit_pair(smem_u32(&acc_full[a]));
+        else commit(smem_u32(&acc_full[a]));
+        if (++a == 2) { a = 0; acc_turn ^= 1; }
       }
+      if (!ok) give_up();
     }
   } else {
-    const int quarter = warp & 3;  // the TMEM lanes this warp may read
-    float* patch = staging + (warp - 2) * 32 * 33;
-    const int sub_row = lane >> 3, sub_col = (lane & 7) * 4;
-    int tile_i = 0;
-    for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x, ++tile_i) {
-      const int a = tile_i & 1;
-      const int row0 = tile % tiles_m * I8_BM + quarter * 32, col0 = tile / tiles_m * I8_BN;
-      const float row_scale = row0 + lane < M ? __ldg(scales.rows + row0 + lane) : 0.f;
-      ok = mbar_wait(smem_u32(&acc_full[a]), (tile_i >> 1) & 1, abort_flag);
+    constexpr int CHUNK = 128 / sizeof(TO);  // columns of a patch
+    const int quarter = warp & 3;            // the TMEM lanes this warp may read
+    unsigned char* patch = staging + quarter * Shape::PATCH_BYTES;
+    pdl_wait();
+    int a = 0;
+    uint32_t acc_turn = 0;
+    for (int tile = unit; tile < n_tiles; tile += units) {
+      int m_blk, n_blk;
+      int8_tile_place<TILE_ROWS>(tile, tiles_m, tiles_n, m_blk, n_blk);
+      const int row0 = m_blk * TILE_ROWS + rank * I8_BM + quarter * 32, col0 = n_blk * BN;
+      const float row_scale = row0 + lane < M ? scales.rows[row0 + lane] : 0.f;
+      float* by_column = factors + a * 2 * BN;
+      for (int i = (int)threadIdx.x - 96; i < BN; i += 128) {
+        const int n = min(col0 + i, N - 1);
+        by_column[i] = scales.columns[n];
+        by_column[BN + i] = scales.bias != nullptr ? scales.bias[n] : 0.f;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // (the set of the tile before last is not read any more)
+      ok = mbar_wait(smem_u32(&acc_full[a]), acc_turn, abort_flag);
       if (!ok) break;
       fence_after();
-      const uint32_t tmem_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + a * I8_BN;
+      const uint32_t tmem_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + a * BN;
 #pragma unroll 1
-      for (int c = 0; c < I8_BN; c += 32) {
-        const int col = col0 + c + sub_col;
-        float factor[4], bias[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          factor[e] = col + e < N ? __ldg(scales.columns + col + e) : 0.f;
-          bias[e] = scales.bias != nullptr && col + e < N ? __ldg(scales.bias + col + e) : 0.f;
-        }
+      for (int c = 0; c < BN; c += 32) {
         uint32_t v[32];
         tmem_ld32(v, tmem_row + c);
         tmem_wait_ld();
+        float value[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) patch[lane * 33 + j] = __int2float_rn((int)v[j]) * row_scale;
-        __syncwarp();
+        for (int j = 0; j < 32; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(by_column + c + j), b = *reinterpret_cast<const float4*>(by_column + BN + c + j);
+          value[j] = fmaf(__int2float_rn((int)v[j]) * row_scale, f.x, b.x);
+          value[j + 1] = fmaf(__int2float_rn((int)v[j + 1]) * row_scale, f.y, b.y);
+          value[j + 2] = fmaf(__int2float_rn((int)v[j + 2]) * row_scale, f.z, b.z);
+          value[j + 3] = fmaf(__int2float_rn((int)v[j + 3]) * row_scale, f.w, b.w);
+        }
+        if (by_tma) {
+          const int part = c % CHUNK;  // where in the patch
+          if (part == 0) {
+            tma_stores_read();
+            __syncwarp();
+          }
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int row = row0 + it * 4 + sub_row;
-          const float* src = patch + (it * 4 + sub_row) * 33 + sub_col;
-          if (row < M) {
-            TO* dst = out + (size_t)row * ldo + col;
+          for (int j = 0; j < 32; j += 16 / sizeof(TO)) {
+            const int u = (part + j) * (int)sizeof(TO) / 16;
+            *reinterpret_cast<uint4*>(patch + lane * 128 + ((u ^ (lane & 7)) << 4)) = int8_unit<TO>(value, j);
+          }
+          if (part + 32 == CHUNK) {
+            fence_to_async();
+            __syncwarp();
+            if (elect_one() && row0 < M && col0 + c - part < N) tma_store_2d(&map_out, col0 + c - part, row0, smem_u32(patch), MODE == 1);
+          }
+        } else {
+          float* square = reinterpret_cast<float*>(patch);  // 32 rows, 33 floats apart
+          __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (col + e < N) {
-                const float value = fmaf(src[e], factor[e], bias[e]);
-                dst[e] = from_float<TO>(MODE == 1 ? to_float(dst[e]) + value : value);
+          for (int j = 0; j < 32; ++j) square[lane * 33 + j] = value[j];
+          __syncwarp();
+          const int col = col0 + c + lane, rows = min(32, M - row0);
+          TO* dst = out + (size_t)row0 * ldo + col;
+          if (col < N) {
+            if (MODE == 0 && rows == 32) {
+#pragma unroll
+              for (int r = 0; r < 32; ++r, dst += ldo) *dst = from_float<TO>(square[r * 33 + lane]);
+            } else {
+#pragma unroll 1
+              for (int r0 = 0; r0 < rows; r0 += 8) {
+                // what is added into is asked for before the first store, which might be to the same memory
+                float old[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) old[r] = MODE == 1 && r0 + r < rows ? to_float(dst[(size_t)(r0 + r) * ldo]) : 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                  const float sum = square[min(r0 + r, 31) * 33 + lane];
+                  if (r0 + r < rows) dst[(size_t)(r0 + r) * ldo] = from_float<TO>(MODE == 1 ? old[r] + sum : sum);
+                }
               }
+            }
           }
         }
-        __syncwarp();
       }
       fence_before();
-      mbar_arrive(smem_u32(&acc_empty[a]));
+      if (PAIR) mbar_arrive_remote(first_block_address(smem_u32(&acc_empty[a])));
+      else mbar_arrive(smem_u32(&acc_empty[a]));
+      if (++a == 2) { a = 0; acc_turn ^= 1; }
     }
+    tma_stores_done();
+    if (!ok && lane == 0) give_up();
   }
-  if (!ok) { *abort_flag = 1; if (error_flag != nullptr) atomicExch(error_flag, 6); }
 
   fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (PAIR) cluster_sync();  // neither block leaves while the other may still arrive on its barriers or read its shared memory
+  if (warp == 2) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN));
   }
 }
 
-template <int MODE, typename TO>
-int launch_gemm_int8(void* out, const CUtensorMap& map_x, const CUtensorMap& map_w, int M, int N, int K, int ldo,
-                     const Int8Scales& scales, int sm_count, int* error_flag, cudaStream_t stream) {
-  constexpr auto kernel = gemm_int8_kernel<MODE, TO>;
-  const cudaError_t err = allow_shared_memory_once<kernel>(I8_SMEM);
+// A product's operands as the launchers pass them on.
+struct Int8Product {
+  void* out;
+  const void* codes;
+  const void* w;
+  int M, N, K, ldx, ldw, ldo;
+  Int8Scales scales;
+  int sm_count;
+  int* error_flag;
+};
+
+template <int MODE, bool PAIR, int BN, typename TO>
+int launch_gemm_int8_tiled(const Int8Product& p, cudaStream_t stream) {
+  using Shape = Int8Shape<PAIR, BN>;
+  constexpr auto kernel = gemm_int8_kernel<MODE, PAIR, BN, TO>;
+  const cudaError_t err = allow_shared_memory_once<kernel>(Shape::SMEM);
   if (err != cudaSuccess) return (int)err;
-  const long long tiles = (long long)((M + I8_BM - 1) / I8_BM) * ((N + I8_BN - 1) / I8_BN);
-  launch_kernel_alone(kernel, dim3((unsigned)(tiles < sm_count ? tiles : sm_count)), dim3(I8_THREADS), (size_t)I8_SMEM, stream, map_x,
-                      map_w, (TO*)out, M, N, K, ldo, scales, error_flag);
+  CUtensorMap map_x, map_w, map_out = {};
+  if (!make_map_int8_2d(&map_x, p.codes, p.M, p.K, p.ldx, I8_BM) || !make_map_int8_2d(&map_w, p.w, p.N, p.K, p.ldw, Shape::B_ROWS))
+    return XRT_ERR_UNSUPPORTED;
+  const int by_tma = ((uintptr_t)p.out & 15) == 0 && (size_t)p.ldo * sizeof(TO) % 16 == 0;
+  if (by_tma && !make_map_result_2d(&map_out, p.out, p.M, p.N, p.ldo, sizeof(TO))) return XRT_ERR_UNSUPPORTED;
+  constexpr int tile_rows = (PAIR ? 2 : 1) * I8_BM;
+  const long long tiles = (long long)((p.M + tile_rows - 1) / tile_rows) * ((p.N + BN - 1) / BN);
+  const int units = PAIR ? p.sm_count / 2 : p.sm_count;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(tiles < units ? tiles : units) * (PAIR ? 2 : 1));
+  config.blockDim = dim3(I8_THREADS);
+  config.dynamicSmemBytes = Shape::SMEM;
+  config.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  int n_attrs = 0;
+  if (pdl_enabled()) {  // (a block fills its multiprocessor's shared memory: placed early, none shares one)
+    attrs[n_attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[n_attrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (PAIR) {
+    attrs[n_attrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[n_attrs].val.clusterDim.x = 2; attrs[n_attrs].val.clusterDim.y = 1; attrs[n_attrs++].val.clusterDim.z = 1;
+  }
+  config.attrs = attrs;
+  config.numAttrs = n_attrs;
+  cudaLaunchKernelEx(&config, kernel, map_x, map_w, map_out, (TO*)p.out, by_tma, p.M, p.N, p.K, p.ldo, p.scales, p.error_flag);
   return launch_status();
+}
+
+// The tile: 0 pairs of 256 x 256, 1 pairs of 256 x 128, 2 single blocks of 128 x 256, 3 of 128 x 128: the least of what it takes
+// to begin and end, and the longer of the rounds of tiles (microseconds a 128-wide slab of K) and the operands from memory,
+// as measured on a B200 with the operands in memory.  Microseconds (0 / 1 / 2 / 3): 256 rows of 6,144 outputs, 4,096 inputs
+// 15.5 / 11.5 / 17.1 / 11.8; 333 of 6,144, 4,096 16.4 / 16.3 / 17.0 / 12.0; 512 of 4,096, 14,336 39.1 / 25.5 / 44.6 / 28.9;
+// 8,192 of 28,672, 4,096 546 / 686 / 608 / 851 (3,527 TOP/s).
+static int int8_form(const Int8Product& p) {
+  constexpr int rows[4] = {256, 256, 128, 128}, columns[4] = {256, 128, 256, 128};
+  constexpr double slab_us[4] = {0.281, 0.168, 0.35, 0.21}, ends_us[4] = {6.5, 6.1, 5.9, 5.1};
+  const double memory_us = ((double)p.M + p.N) * p.K / 5e6;
+  const long long slabs = (p.K + I8_BK - 1) / I8_BK;
+  int best = 0;
+  double least = 0;
+  for (int form = 0; form < 4; ++form) {
+    const long long tiles = (long long)((p.M + rows[form] - 1) / rows[form]) * ((p.N + columns[form] - 1) / columns[form]);
+    const int units = rows[form] == 256 ? p.sm_count / 2 : p.sm_count;
+    const double walk_us = (double)((tiles + units - 1) / units * slabs) * slab_us[form];
+    const double cost = ends_us[form] + (walk_us > memory_us ? walk_us : memory_us);
+    if (form == 0 || cost < least) { least = cost; best = form; }
+  }
+  return best;
+}
+
+template <int MODE, typename TO>
+int launch_gemm_int8(const Int8Product& p, cudaStream_t stream) {
+  const int form = int8_form(p);
+  if (form == 0) return launch_gemm_int8_tiled<MODE, true, 256, TO>(p, stream);
+  if (form == 1) return launch_gemm_int8_tiled<MODE, true, 128, TO>(p, stream);
+  if (form == 2) return launch_gemm_int8_tiled<MODE, false, 256, TO>(p, stream);
+  return launch_gemm_int8_tiled<MODE, false, 128, TO>(p, stream);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -197,7 +393,7 @@ int launch_gemm_int8(void* out, const CUtensorMap& map_x, const CUtensorMap& map
 // warp 4 owns the TMEM and issues the MMAs; warps 5-8 bring the accumulators to shared memory, where all warps finish them.  A
 // kernel this short also pays for every instruction that it meets for the first time (its code comes from the L2): the
 // finish is one short loop, and while warps 5-8 wait they walk it once into a place that nobody reads.
-constexpr int FEW_MAX_ROWS = 128, FEW_MAX_SPLITS = 8, FEW_MAX_STAGES = 24;
+constexpr int FEW_MAX_ROWS = 128, FEW_MAX_SPLITS = 4, FEW_MAX_STAGES = 24;
 constexpr int FEW_PRODUCERS = 4;
 constexpr int FEW_THREADS = 32 * (FEW_PRODUCERS + 1 + 4);
 constexpr int FEW_TAIL_BYTES = 512 + 4 * (FEW_MAX_ROWS + 2 * 256);  // barriers, flags, a place that nobody reads; scales, biases
@@ -461,12 +657,13 @@ static int few_shared_bytes(const FewShape& s) {
 
 // The tile, the parts of K and the ring of a product, from what was measured on a B200 (148 multiprocessors).
 //
-// Up to 128 weight rows a multiprocessor, one block each: the time is the longer of W from memory (6.3 TB/s in all, 110 GB/s
-// into one multiprocessor) and a block's walk over its slabs (0.15 us each, or their bytes at 110 GB/s), a third of the
-// shorter, and what it takes to begin and end: 2 us, and where the parts of a tile meet 0.8 us more and 0.4 us for each
-// 1,000 sums that a block sends.  Clusters of 3 and 4 do not fill the device (45 and 33 are held; many fewer of 3 at once in
-// practice).  Microseconds, chosen against the next best number of parts: 8 rows of 4,096 outputs, 4,096 inputs 5.9 (4 parts; 2: 6.0,
-// 1: 7.8); 6,144, 4,096 7.1 (2; 4: 7.5); 4,096, 14,336 12.4 (4; 3: 12.8); 64 of 2,048, 2,048 4.8 (2; 4: 5.2).
+// Up to 128 weight rows a multiprocessor, one block each, the cheapest of some tiles and numbers of parts by this sum of
+// microseconds (fitted to the times of 65 products of 1 to 128 rows with every one of them: on average 2.3 percent above the
+// best): the longer of W from memory (6.3 TB/s in all, 0.11 TB/s into one multiprocessor, less with copies of fewer than 64
+// rows) and a block's walk over its slabs (0.15 each, or their bytes at 0.11 TB/s), half of the shorter, 0.01 a block, 0.2 for
+// each 1,000 sums that a block finishes, 0.3 where the parts of a tile meet and 0.3 for tiles of two MMAs.  The device does not
+// hold clusters of 3 and 4 on all multiprocessors.  Chosen against other numbers of parts: 8 rows of 4,096 outputs, 14,336
+// inputs 12.5 (4 parts; 3: 12.8, 1: 21); 6,144, 4,096 7.5 (2; 4: 7.4, 1: 8.5); 64 of 2,048, 2,048 4.8 (2; 4: 5.2).
 //
 // More weight rows than that: K is not split.  Two blocks a multiprocessor with a ring of four slabs each, if their
 // tiles make one round of it or even tiles of 256 rows do not (8 rows of 28,672 outputs, 4,096 inputs 19.1 against 19.8 with one
@@ -480,53 +677,64 @@ static void plan_few(FewShape& s, int K, int sm_count) {
   if (even_rows(sm_count) <= 128) {
     double best = 0;
     s.splits = 0;
-    for (int splits = 1; splits <= 4 && (splits == 1 || slabs >= 4 * splits); ++splits) {
-      const int blocks = splits <= 2 ? sm_count : splits == 3 ? sm_count * 4 / 5 : sm_count * 8 / 9;
+    for (int splits = 1; splits <= FEW_MAX_SPLITS && (splits == 1 || slabs >= 2 * splits); ++splits) {
+      const int blocks = splits <= 2 ? sm_count : sm_count * 22 / 25;
       if (blocks < splits) break;
       const int even = even_rows(blocks / splits);
       for (int rows : {32, 64, 96, 128, even}) {
         if (rows > 256 || rows < even) continue;
         const int used = (s.N + rows - 1) / rows * splits;
-        const double rate = used * 0.11e6 < 6.3e6 ? used * 0.11e6 : 6.3e6, slab_us = (rows + s.M) * 128 / 110e3;
-        const double memory_us = (double)s.N * K / rate;
+        const double into = used * 0.11e6 * (rows < 64 ? rows / 64.0 : 1.0), slab_us = (rows + s.M) * 128 / 0.11e6;
+        const double memory_us = (double)s.N * K / (into < 6.3e6 ? into : 6.3e6);
         const double walk_us = (slabs + splits - 1) / splits * (slab_us > 0.15 ? slab_us : 0.15);
-        const double longer = memory_us > walk_us ? memory_us : walk_us;
-        const double cost = longer + 0.3 * (memory_us + walk_us - longer) + (splits > 1 ? 0.8 + 0.4e-3 * rows * s.M : 0.0);
+        const double cost = (memory_us > walk_us ? memory_us + 0.5 * walk_us : walk_us + 0.5 * memory_us) + 0.01 * used +
+                            0.2e-3 * rows * s.M + (splits > 1 ? 0.3 : 0.0) + (rows > 128 ? 0.3 : 0.0);
         if (s.splits == 0 || cost < best) { best = cost; s.splits = splits; s.rows = rows; }
       }
     }
   } else {
-    const int two_most = 220 - s.nb;  // weight rows that leave room for four slabs
+    const int two_most = 212 - s.nb;  // weight rows that leave room for four slabs
     const int two_rounds = (s.N + 2 * sm_count * two_most - 1) / (2 * sm_count * two_most);
     const int one_rounds = (s.N + sm_count * 256 - 1) / (sm_count * 256);
     const bool two = two_rounds == 1 || one_rounds > 1;
     s.splits = 1;
-    s.rows = two ? even_rows(2 * sm_count * two_rounds) : even_rows(sm_count);
+    s.rows = even_rows(two ? 2 * sm_count * two_rounds : sm_count);
     if (two) limit = FEW_SHARED_TWO;
   }
-  // slabs a stage: as many as leave a ring of three stages
-  for (s.slabs = 4; s.slabs > 1; s.slabs /= 2) {
-    s.stages = 3;
-    if (few_shared_bytes(s) <= limit) break;
-  }
-  s.k_iters = (slabs + s.slabs - 1) / s.slabs;
-  const int share = (s.k_iters + s.splits - 1) / s.splits;
+  // The ring: slabs a stage as many as leave three stages (or all that a block walks).  The producers, which take
+  // every fourth slab each, need a ring of four slabs if it turns: two blocks a multiprocessor or parts of K that leave no
+  // room for that are given up.
   for (;;) {
+    for (s.slabs = 4; s.slabs > 1; s.slabs /= 2) {
+      const int walked = ((slabs + s.slabs - 1) / s.slabs + s.splits - 1) / s.splits;
+      s.stages = walked < 3 ? walked : 3;
+      if (few_shared_bytes(s) <= limit && slabs >= s.slabs * s.splits) break;
+    }
+    s.k_iters = (slabs + s.slabs - 1) / s.slabs;
+    const int share = (s.k_iters + s.splits - 1) / s.splits;
     s.stages = FEW_MAX_STAGES;
     while (s.stages > 1 && few_shared_bytes(s) > limit) --s.stages;
-    // the producers, which take every fourth slab each, need a ring of four slabs if it turns
-    if (s.stages * s.slabs >= FEW_PRODUCERS || s.stages >= share || limit == FEW_SHARED_ONE) break;
-    limit = FEW_SHARED_ONE;
+    if (s.stages > share) s.stages = share;
+    if ((s.stages * s.slabs >= FEW_PRODUCERS || s.stages == share) && few_shared_bytes(s) <= limit) break;
+    if (limit == FEW_SHARED_TWO) limit = FEW_SHARED_ONE;
+    else if (s.splits > 1) --s.splits;
+    else s.rows = (s.rows / 2 + 7) / 8 * 8;  // (no product of this library's sizes comes here)
   }
-  if (s.stages > share) s.stages = share;
 }
 
 template <int MODE, typename TO>
-int launch_gemm_int8_few(void* out, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewShape& shape, const Int8Scales& scales,
-                         int* error_flag, cudaStream_t stream) {
+int launch_gemm_int8_few(const Int8Product& p, int constant_weight, cudaStream_t stream) {
   constexpr auto kernel = gemm_int8_few_kernel<MODE, TO>;
   const cudaError_t err = allow_shared_memory_once<kernel>(FEW_SHARED_ONE);
   if (err != cudaSuccess) return (int)err;
+  FewShape shape = {};
+  shape.M = p.M; shape.N = p.N; shape.ldo = p.ldo;
+  shape.nb = (p.M + 15) / 16 * 16;
+  shape.early = constant_weight;
+  plan_few(shape, p.K, p.sm_count);
+  CUtensorMap map_w, map_x;
+  if (!make_map_int8_2d(&map_x, p.codes, p.M, p.K, p.ldx, shape.nb) || !make_map_int8_2d(&map_w, p.w, p.N, p.K, p.ldw, shape.rows))
+    return XRT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)((shape.N + shape.rows - 1) / shape.rows) * shape.splits);
   config.blockDim = dim3(FEW_THREADS);
@@ -542,7 +750,7 @@ int launch_gemm_int8_few(void* out, const CUtensorMap& map_w, const CUtensorMap&
   attrs[n_attrs].val.clusterDim.x = shape.splits; attrs[n_attrs].val.clusterDim.y = 1; attrs[n_attrs++].val.clusterDim.z = 1;
   config.attrs = attrs;
   config.numAttrs = n_attrs;
-  cudaLaunchKernelEx(&config, kernel, map_w, map_x, (TO*)out, shape, scales, error_flag);
+  cudaLaunchKernelEx(&config, kernel, map_w, map_x, (TO*)p.out, shape, p.scales, p.error_flag);
   return launch_status();
 }
 
@@ -559,29 +767,12 @@ XRT_EXPORT int xrt_gemm_int8(void* out, const void* codes, const float* scales, 
   if (mode == 1 && out_dtype != XRT_F32) return XRT_ERR_ARGUMENT;
   if (ldx % 16 != 0 || ldw % 16 != 0 || ((uintptr_t)codes & 15) || ((uintptr_t)w & 15)) return XRT_ERR_UNSUPPORTED;
   if (M == 0) return XRT_OK;
-  const int sm_count = xrt::multiprocessors();
-  if (sm_count <= 0) return XRT_ERR_UNSUPPORTED;
-  CUtensorMap map_x, map_w;
-  const xrt::Int8Scales factors{scales, w_scales, bias};
-  if (M <= xrt::FEW_MAX_ROWS) {
-    xrt::FewShape shape = {};
-    shape.M = M; shape.N = N; shape.ldo = ldo;
-    shape.nb = (M + 15) / 16 * 16;
-    shape.early = constant_weight;
-    xrt::plan_few(shape, K, sm_count);
-    if (!xrt::sm100::make_map_int8_2d(&map_x, codes, M, K, ldx, shape.nb) ||
-        !xrt::sm100::make_map_int8_2d(&map_w, w, N, K, ldw, shape.rows))
-      return XRT_ERR_UNSUPPORTED;
-    if (mode == 1) return xrt::launch_gemm_int8_few<1, float>(out, map_w, map_x, shape, factors, error_flag, stream);
-    XRT_DISPATCH_DTYPE(out_dtype, TO, {
-      return xrt::launch_gemm_int8_few<0, TO>(out, map_w, map_x, shape, factors, error_flag, stream);
-    });
-  }
-  if (!xrt::sm100::make_map_int8_2d(&map_x, codes, M, K, ldx, 128) || !xrt::sm100::make_map_int8_2d(&map_w, w, N, K, ldw, 128))
-    return XRT_ERR_UNSUPPORTED;
+  const xrt::Int8Product p{out, codes, w, M, N, K, ldx, ldw, ldo, {scales, w_scales, bias}, xrt::multiprocessors(), error_flag};
+  if (p.sm_count <= 1) return XRT_ERR_UNSUPPORTED;
+  const bool few = M <= xrt::FEW_MAX_ROWS;
   if (mode == 1)
-    return xrt::launch_gemm_int8<1, float>(out, map_x, map_w, M, N, K, ldo, factors, sm_count, error_flag, stream);
+    return few ? xrt::launch_gemm_int8_few<1, float>(p, constant_weight, stream) : xrt::launch_gemm_int8<1, float>(p, stream);
   XRT_DISPATCH_DTYPE(out_dtype, TO, {
-    return xrt::launch_gemm_int8<0, TO>(out, map_x, map_w, M, N, K, ldo, factors, sm_count, error_flag, stream);
+    return few ? xrt::launch_gemm_int8_few<0, TO>(p, constant_weight, stream) : xrt::launch_gemm_int8<0, TO>(p, stream);
   });
 }

@@ -60,6 +60,22 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
                ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
 }
 
+// A tile of shared memory into a two-dimensional tensor map (or, with `add`, added into it, float32), in a group of this thread's;
+// writes of the tile by other threads must have been fenced (fence_to_async) before.  c0 as for the loads.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src, bool add) {
+  if (add)
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(map), "r"(c0), "r"(c1), "r"(src) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(map), "r"(c0), "r"(c1), "r"(src) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Until this thread's stores have read their shared memory, or until they are done.
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // A cache policy for data that is read once (a weight, a cache of keys): its lines are the first
 // to leave the L2, so that what is read again (code, activations, the residual) stays there.
 __device__ __forceinline__ uint64_t policy_evict_first() {
@@ -220,7 +236,21 @@ inline bool make_map_bf16_2d(CUtensorMap* map, const void* base, long long rows,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The same over 8-bit integers [rows, cols] with row stride `ld` bytes (a multiple of 16): boxes of `box_rows` rows x 128
+// A map over a row-major result [rows, cols] of `size` bytes an element (2: bfloat16, 4: float32) with row stride `ld` elements:
+// boxes of 32 rows x 128 bytes, 128-byte swizzle.
+inline bool make_map_result_2d(CUtensorMap* map, void* base, long long rows, long long cols, long long ld, int size) {
+  TensorMapEncodeFn encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32u};
+  const cuuint32_t elem[2] = {1u, 1u};
+  return encode(map, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, base, dims, strides, box, elem,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A map over 8-bit integers [rows, cols] with row stride `ld` bytes (a multiple of 16): boxes of `box_rows` rows x 128
 // columns.  What a box has beyond rows or cols arrives as zeros.
 inline bool make_map_int8_2d(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_rows) {
   TensorMapEncodeFn encode = tensor_map_encoder();

@@ -77,6 +77,48 @@ def test_rows_whose_addresses_allow_only_single_values(rows, width):
     check_codes(codes, scales, whole, x.double(), 0.0)
 
 
+# more rows than blocks: rows that come through a ring, at every 16-byte phase, with rows that begin and end anywhere
+MANY = [(3000, 33), (1500, 1600), (1300, 3001), (700, 4096), (1203, 4099), (333, 8190), (150, 14337), (400, 16384), (450, 25600),
+        (449, 25001), (301, 26000), (300, 30000), (152, 33000)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width", MANY)
+def test_many_rows(rows, width, dtype):
+    x = normal(rows, width, seed=70, dtype=DT[dtype])
+    x[rows // 2] = 0
+    x[1, width - 1] = float("nan")
+    codes, scales, whole = room(rows, width)
+    ops().quantize_rows(codes, scales, x)
+    assert bool(torch.isnan(scales[1])) and not bool(codes[1].any())
+    keep = torch.arange(rows, device=DEV) != 1
+    check_codes(codes[keep], scales[keep], whole, x[keep].double(), 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("rows,width", [(1203, 1999), (700, 4096), (333, 7005), (301, 14336), (160, 12800), (155, 12801)])
+def test_many_gates(rows, width, act, dtype):
+    gate_up = (normal(rows, 2 * width, seed=71) * 3).to(DT[dtype])
+    codes, scales, whole = room(rows, width)
+    ops().swiglu_int8(codes, scales, gate_up, act)
+    check_codes(codes, scales, whole, gate_formula(gate_up, act), 2.0 ** -15)
+
+
+@pytest.mark.parametrize("add", [None, "float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width", [(1203, 1999), (1000, 2048), (700, 4096), (613, 4099), (333, 8190), (300, 13000), (170, 20001)])
+def test_many_norms(rows, width, add):
+    x = normal(rows, width, seed=72)
+    w = 1 + 0.1 * normal(width, seed=73)
+    more = None if add is None else normal(rows, width, seed=74).to(DT[add])
+    s = x if add is None else x + more.float()
+    want = s.double() / torch.sqrt((s.double() ** 2).mean(dim=1, keepdim=True) + 3e-6) * w.double()
+    codes, scales, whole = room(rows, width)
+    ops().rmsnorm_int8(codes, scales, x, w, 3e-6, add=more)
+    check_codes(codes, scales, whole, want, 2.0 ** -19)
+    assert torch.equal(x, s)
+
+
 def gate_formula(gate_up, act):
     g, u = gate_up.double().chunk(2, dim=1)
     if act == "silu":

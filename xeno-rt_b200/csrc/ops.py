@@ -91,9 +91,9 @@ _SIGNATURES = {
     "xrt_recurrence_gates": [_P, _P, _P, _P, _P, _I, _P],
     "xrt_recurrence_scan": [_P, _P, _I, _I, _P],
     "xrt_recurrence_step": [_P, _P, _P, _P, _P, _P, _I, _P],
-    "xrt_quantize_rows": [_P, _P, _P, _I, _I, _I, _I, _P],
-    "xrt_swiglu_int8": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P],
-    "xrt_rmsnorm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _P],
+    "xrt_quantize_rows": [_P, _P, _P, _I, _I, _I, _I, _P, _P],
+    "xrt_swiglu_int8": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P],
+    "xrt_rmsnorm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _P, _P],
     "xrt_gemm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "xrt_fill_normal": [_P, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_double, _I, _P],
     "xrt_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P],
@@ -1729,7 +1729,7 @@ def _error_flag_pointer(index: int) -> int:
     """A device's error flag for a launch; 0 (the kernel reports nothing) where it would have to be made inside a capture."""
     flag = _error_flags.get(index)
     if flag is None:
-        if torch.cuda.is_current_stream_capturing():
+        if index < 0 or torch.cuda.is_current_stream_capturing():
             return 0
         flag = error_flag(torch.device("cuda", index))
     return flag.data_ptr()
@@ -1761,7 +1761,8 @@ def quantize_rows(codes, scales, x) -> None:
         raise KernelError(f"{what}: x must be [rows, width]")
     n, width = x.shape
     ld = _codes(codes, "codes", what, n, width)
-    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), n, width, ld, _code(x.dtype))
+    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), n, width, ld, _code(x.dtype),
+            _error_flag_pointer(x.get_device()))
     _run_int8(what, (x, codes, scales), "xrt_quantize_rows", args)
 
 
@@ -1778,7 +1779,7 @@ def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
     ld = _codes(codes, "codes", what, n, width)
     options = gate.options(width)
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), n, width, ld, _code(gate_up.dtype),
-            code, options)
+            code, options, _error_flag_pointer(gate_up.get_device()))
     _run_int8(what, (gate_up, codes, scales, gate.bias), "xrt_swiglu_int8", args)
 
 
@@ -1800,7 +1801,7 @@ def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None) -> No
     ld = _codes(codes, "codes", what, n, width)
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),
             _ptr(out, "out", torch.float32), _ptr(weight, "weight"), n, width, ld, float(eps),
-            0 if add is None else _code(add.dtype), _code(weight.dtype))
+            0 if add is None else _code(add.dtype), _code(weight.dtype), _error_flag_pointer(x.get_device()))
     _run_int8(what, (x, codes, scales, weight, add, out), "xrt_rmsnorm_int8", args)
 
 
@@ -1833,5 +1834,5 @@ def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = Fals
     args = (out.data_ptr(), codes.data_ptr(), _vector(scales, "scales", what, m), weight.data_ptr(),
             _vector(weight_scales, "weight_scales", what, n), 0 if bias is None else _vector(bias, "bias", what, n), m, n, k,
             ldx, ldw, out_distance if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0,
-            _error_flag_pointer(out.get_device()) if out.is_cuda else 0)
+            _error_flag_pointer(out.get_device()))
     _run_int8(what, (out, codes, scales, weight, weight_scales, bias), "xrt_gemm_int8", args)

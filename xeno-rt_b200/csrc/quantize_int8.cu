@@ -6,14 +6,16 @@
 // A row of zeros has codes 0 and the smallest scale.  A row with a NaN or an infinity has codes 0 and the scale NaN, so that
 // every product with it is NaN.  Sums, statistics and y are 32-bit; the codes are the only rounding to fewer bits.
 //
-// One block a row, the row in registers: read once with loads that are all in flight together, one meeting of the block
-// (the norm's sum of squares and the largest |s w| are found in the same pass, since the factor 1 / rms is the
+// One block a row, the row in registers: read once, one meeting of the block (the norm's sum of squares and the largest |s w| are found in the same pass, since the factor 1 / rms is the
 // same for the whole row), codes written once.  The largest absolute value is found on the bits: for numbers without
 // a sign their order is that of the integers, and every NaN lies above infinity.
-// Rows beyond what 1,024 threads hold are walked twice.
+//
+// Few rows (steps): a block a row, its loads all in flight together.  More rows than blocks: blocks take every so many-th
+// row from a ring in shared memory that bulk copies fill ahead (quantize_int8_ring_kernel), so that the memory is asked for the
+// next rows while a block meets.  Rows beyond what 1,024 threads hold are walked twice.
 #include <type_traits>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace xrt {
 
@@ -88,8 +90,15 @@ __device__ __forceinline__ void store_codes(int8_t* p, const float (&y)[VEC], fl
 template <typename T>
 struct PlainRows {
   static constexpr bool NORMED = false;
+  static constexpr bool GATED = false;
+  static constexpr int STREAMS = 1;  // what a row consists of in memory: pieces of `length` elements of From<i>
+  template <int I> using From = T;
   const T* x;
+  template <int I> __host__ __device__ __forceinline__ const T* from() const { return x; }
+  __host__ __device__ __forceinline__ static int length(int width) { return width; }
   __device__ __forceinline__ void wait() { pdl_wait(x); }
+  // the values from a row's streams where those lie in shared memory
+  template <int VEC, class READ> __device__ __forceinline__ void read(int c, int, const READ& get, float (&v)[VEC]) const { get.template operator()<0, VEC>(c, v); }
   template <int VEC> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
   template <int VEC, bool AGAIN> __device__ __forceinline__ void load(int row, int c, int width, float (&v)[VEC]) const {
     load_some<VEC>(x + (size_t)row * width + c, v);
@@ -101,15 +110,15 @@ struct PlainRows {
 template <typename T>
 struct GatedRows {
   static constexpr bool NORMED = false;
+  static constexpr bool GATED = true;
+  static constexpr int STREAMS = 1;
+  template <int I> using From = T;
   const T* gate_up;  // [rows, 2 * width]
   RowScale gate;
+  template <int I> __host__ __device__ __forceinline__ const T* from() const { return gate_up; }
+  __host__ __device__ __forceinline__ static int length(int width) { return 2 * width; }
   __device__ __forceinline__ void wait() { pdl_wait(gate_up); }
-  template <int VEC> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
-  template <int VEC, bool AGAIN> __device__ __forceinline__ void load(int row, int c, int width, float (&v)[VEC]) const {
-    const T* p = gate_up + (size_t)row * 2 * width + c;
-    float u[VEC];
-    load_some<VEC>(p, v);
-    load_some<VEC>(p + width, u);
+  template <int VEC> __device__ __forceinline__ void gated(float (&v)[VEC], float (&u)[VEC], int c) const {
     // the fast exponential and division, as for a bfloat16 result: 8 bits are kept
     if (gate.gate_act == 1) {
       // 0.5 g (1 + tanh(z)) = g sigmoid(2 z), which loses nothing where tanh(z) is near -1: alone in its row, such a
@@ -122,6 +131,20 @@ struct GatedRows {
       gated_units<__nv_bfloat16, VEC, true>(v, u, c, gate);
     }
   }
+  template <int VEC, class READ> __device__ __forceinline__ void read(int c, int width, const READ& get, float (&v)[VEC]) const {
+    float u[VEC];
+    get.template operator()<0, VEC>(c, v);
+    get.template operator()<0, VEC>(width + c, u);
+    gated<VEC>(v, u, c);
+  }
+  template <int VEC> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
+  template <int VEC, bool AGAIN> __device__ __forceinline__ void load(int row, int c, int width, float (&v)[VEC]) const {
+    const T* p = gate_up + (size_t)row * 2 * width + c;
+    float u[VEC];
+    load_some<VEC>(p, v);
+    load_some<VEC>(p + width, u);
+    gated<VEC>(v, u, c);
+  }
   template <int VEC, bool AGAIN>
   __device__ __forceinline__ void settle(int, int, int, const float (&)[VEC], float (&)[VEC], float&) const {}
 };
@@ -133,6 +156,23 @@ template <typename TA, typename TW>
 struct NormedRows {
   static constexpr bool NORMED = true;
   static constexpr bool ADDS = !std::is_same<TA, Nothing>::value;
+  static constexpr bool GATED = false;
+  static constexpr int STREAMS = ADDS ? 2 : 1;
+  template <int I> using From = std::conditional_t<I == 0, float, TA>;
+  template <int I> __host__ __device__ __forceinline__ const From<I>* from() const {
+    if constexpr (I == 0) return x;
+    else return add;
+  }
+  __host__ __device__ __forceinline__ static int length(int width) { return width; }
+  template <int VEC, class READ> __device__ __forceinline__ void read(int c, int, const READ& get, float (&v)[VEC]) const {
+    get.template operator()<0, VEC>(c, v);
+    if constexpr (ADDS) {
+      float a[VEC];
+      get.template operator()<1, VEC>(c, a);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] += a[i];
+    }
+  }
   const float* x;
   const TA* add;
   float* sum;  // may be x
@@ -184,6 +224,41 @@ __device__ __forceinline__ void meet(uint32_t& bits, float& squares, uint32_t (&
   if (NORMED) squares = warp_sum(lane < warps ? sums[lane] : 0.f);
 }
 
+// The scale of a row whose largest value times `factor` is `bits`, and its codes from the values that the threads hold.
+struct RowScaleOf {
+  float factor, scale, inverse;
+  bool broken;
+};
+template <class ROWS>
+__device__ __forceinline__ RowScaleOf scale_of(const ROWS& rows, int width, uint32_t bits, float squares) {
+  RowScaleOf s;
+  s.factor = 1.f;
+  if constexpr (ROWS::NORMED) s.factor = 1.0f / sqrtf(squares / (float)width + rows.eps);
+  const float largest = __uint_as_float(bits) * s.factor;
+  s.broken = !(largest <= 3.402823466e38f);
+  s.scale = s.broken ? __uint_as_float(0x7fc00000u) : fmaxf(largest / CODE_MAX, SMALLEST_SCALE);
+  s.inverse = 1.0f / s.scale;
+  return s;
+}
+template <class ROWS, int VEC, int ITEMS>
+__device__ __forceinline__ void finish_row(int8_t* codes, float* scales, const ROWS& rows, int row, int width, int ld_codes, int stride,
+                                           uint32_t bits, float squares, float (&v)[ITEMS][VEC]) {
+  const RowScaleOf s = scale_of(rows, width, bits, squares);
+  if (threadIdx.x == 0) scales[row] = s.scale;
+  int8_t* dst = codes + (size_t)row * ld_codes;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = (int)threadIdx.x * VEC + i * stride;
+    if (c < width) {
+      if constexpr (ROWS::NORMED) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] *= s.factor;
+      }
+      store_codes<VEC>(dst + c, v[i], s.inverse, s.broken);
+    }
+  }
+}
+
 // ITEMS pieces of VEC values a thread; 0: as many as the row takes, walked twice.
 template <class ROWS, int VEC, int ITEMS>
 __global__ void __launch_bounds__(1024)
@@ -231,37 +306,178 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
     }
   }
   meet<ROWS::NORMED>(bits, squares, most, sums);
-  float factor = 1.f;
-  if constexpr (ROWS::NORMED) factor = 1.0f / sqrtf(squares / (float)width + rows.eps);
-  const float largest = __uint_as_float(bits) * factor;
-  const bool broken = !(largest <= 3.402823466e38f);
-  const float scale = fmaxf(largest / CODE_MAX, SMALLEST_SCALE);
-  const float inverse = 1.0f / scale;
-  if (threadIdx.x == 0) scales[row] = broken ? __uint_as_float(0x7fc00000u) : scale;
-  int8_t* dst = codes + (size_t)row * ld_codes;
   if constexpr (ITEMS > 0) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int c = (int)threadIdx.x * VEC + i * stride;
-      if (c < width) {
-        if constexpr (ROWS::NORMED) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) v[i][j] *= factor;
-        }
-        store_codes<VEC>(dst + c, v[i], inverse, broken);
-      }
-    }
+    finish_row<ROWS, VEC, KEPT>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
   } else {
+    const RowScaleOf s = scale_of(rows, width, bits, squares);
+    if (threadIdx.x == 0) scales[row] = s.scale;
+    int8_t* dst = codes + (size_t)row * ld_codes;
     for (int c = (int)threadIdx.x * VEC; c < width; c += stride) {
       rows.template ahead<VEC>(c, width, w[0]);
       rows.template load<VEC, true>(row, c, width, v[0]);
       rows.template settle<VEC, true>(row, c, width, w[0], v[0], squares);
       if constexpr (ROWS::NORMED) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[0][j] *= factor;
+        for (int j = 0; j < VEC; ++j) v[0][j] *= s.factor;
       }
-      store_codes<VEC>(dst + c, v[0], inverse, broken);
+      store_codes<VEC>(dst + c, v[0], s.inverse, s.broken);
     }
+  }
+}
+
+// The ring.  A stage holds one row's streams, each at its own 16-byte phase: what lies between the first and the last
+// 16-byte boundary of a stream comes by one bulk copy, the few elements outside are put beside it by the lanes of the warp that
+// asks for the copy.
+constexpr int RING_MOST = 8;
+constexpr int RING_LEAST = 6 * 1024;  // bytes of a row: shorter ones are served as well by many small blocks
+// Threads of a block by the values a thread holds: 32 of them need more registers than 1,024 threads have.
+constexpr int ring_threads(int per) { return per > 16 ? 832 : 1024; }
+template <class ROWS, int I>
+__host__ __device__ __forceinline__ int ring_room(int width) {  // of a stream in a stage
+  return (ROWS::length(width) * (int)sizeof(typename ROWS::template From<I>) + 16 + 127) / 128 * 128;
+}
+template <class ROWS>
+__host__ __device__ __forceinline__ int ring_stage(int width) {
+  int bytes = ring_room<ROWS, 0>(width);
+  if constexpr (ROWS::STREAMS == 2) bytes += ring_room<ROWS, 1>(width);
+  return bytes;
+}
+
+template <class ROWS, int I>
+__device__ __forceinline__ const typename ROWS::template From<I>* ring_source(const ROWS& rows, int row, int width) {
+  return rows.template from<I>() + (size_t)row * ROWS::length(width);
+}
+// The bulk copy of a stream of a row to its place in a stage: where it begins and its bytes (0: the stream is too short for one).
+struct RingCopy {
+  uintptr_t begin, lo, hi;
+  __device__ __forceinline__ uint32_t bytes() const { return hi > lo ? (uint32_t)(hi - lo) : 0u; }
+  __device__ __forceinline__ void go(uint32_t place, uint32_t bar) const {
+    if (hi > lo)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   ::"r"(place + (uint32_t)(lo - (begin & ~(uintptr_t)15))), "l"(lo), "r"((uint32_t)(hi - lo)), "r"(bar) : "memory");
+  }
+};
+template <class ROWS, int I>
+__device__ __forceinline__ RingCopy ring_copy(const ROWS& rows, int row, int width) {
+  RingCopy copy;
+  copy.begin = (uintptr_t)ring_source<ROWS, I>(rows, row, width);
+  const uintptr_t end = copy.begin + (size_t)ROWS::length(width) * sizeof(typename ROWS::template From<I>);
+  copy.lo = (copy.begin + 15) & ~(uintptr_t)15;
+  copy.hi = end & ~(uintptr_t)15;
+  return copy;
+}
+// The elements outside that copy, by the lanes of a warp: at most 7 (of 2 bytes) before and 7 behind, or 15 in all.
+template <class ROWS, int I>
+__device__ __forceinline__ void ring_edges(const ROWS& rows, int row, int width, unsigned char* place, int lane) {
+  using T = typename ROWS::template From<I>;
+  const RingCopy copy = ring_copy<ROWS, I>(rows, row, width);
+  const int count = ROWS::length(width), size = (int)sizeof(T);
+  const int before = copy.hi > copy.lo ? (int)(copy.lo - copy.begin) / size : count;
+  const int behind = copy.hi > copy.lo ? count - (int)(copy.hi - copy.begin) / size : 0;
+  const int i = lane < 16 ? lane : count - behind + lane - 16;
+  if (lane < 16 ? lane < before : lane - 16 < behind)
+    reinterpret_cast<T*>(place + (copy.begin & 15))[i] = reinterpret_cast<const T*>(copy.begin)[i];
+}
+
+// A row's elements in its stage.
+template <class ROWS>
+struct RingRow {
+  const unsigned char* first;
+  const unsigned char* second;  // of the streams: the places of element 0
+  template <int I, int VEC>
+  __device__ __forceinline__ void operator()(int c, float (&v)[VEC]) const {
+    load_some<VEC>(reinterpret_cast<const typename ROWS::template From<I>*>(I == 0 ? first : second) + c, v);
+  }
+};
+
+// Rows blockIdx.x, blockIdx.x + gridDim.x, ..
+template <class ROWS, int VEC, int ITEMS>
+__global__ void __launch_bounds__(ring_threads(VEC * ITEMS))
+quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROWS rows, int n, int width, int ld_codes, int stages,
+                          int* error_flag) {
+  using namespace sm100;
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ uint32_t most[2][32];
+  __shared__ float sums[2][32];
+  __shared__ uint64_t full[RING_MOST];
+  __shared__ int abort_flag;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&full[s]), 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const int stride = (int)blockDim.x * VEC, stage_bytes = ring_stage<ROWS>(width), room0 = ring_room<ROWS, 0>(width);
+  const int lane = threadIdx.x & 31;
+  __syncthreads();
+  rows.wait();
+  auto fetch = [&](int row, int s) {  // the first warp
+    unsigned char* place = ring + s * stage_bytes;
+    const uint32_t bar = smem_u32(&full[s]);
+    if constexpr (VEC == 1) {  // (else rows begin and end at 16-byte boundaries)
+      ring_edges<ROWS, 0>(rows, row, width, place, lane);
+      if constexpr (ROWS::STREAMS == 2) ring_edges<ROWS, 1>(rows, row, width, place + room0, lane);
+      __syncwarp();
+    }
+    if (elect_one()) {
+      const RingCopy copy = ring_copy<ROWS, 0>(rows, row, width);
+      if constexpr (ROWS::STREAMS == 2) {
+        const RingCopy second = ring_copy<ROWS, 1>(rows, row, width);
+        mbar_arrive_expect_tx(bar, copy.bytes() + second.bytes());
+        second.go(smem_u32(place) + room0, bar);
+      } else {
+        mbar_arrive_expect_tx(bar, copy.bytes());
+      }
+      copy.go(smem_u32(place), bar);
+    }
+  };
+  if (threadIdx.x < 32)
+    for (int s = 0, row = blockIdx.x; s < stages && row < n; ++s, row += gridDim.x) fetch(row, s);
+  int s = 0, turn = 0, side = 0;
+  for (int row = blockIdx.x; row < n; row += gridDim.x) {
+    if (!mbar_wait(smem_u32(&full[s]), turn, &abort_flag)) {
+      abort_flag = 1;
+      if (error_flag != nullptr) atomicExch(error_flag, 7);
+    }
+    const unsigned char* place = ring + s * stage_bytes;
+    RingRow<ROWS> from{place, place + room0};
+    if constexpr (VEC == 1) {
+      from.first += (uintptr_t)ring_source<ROWS, 0>(rows, row, width) & 15;
+      if constexpr (ROWS::STREAMS == 2) from.second += (uintptr_t)ring_source<ROWS, 1>(rows, row, width) & 15;
+    }
+    float v[ITEMS][VEC], squares = 0.f;
+    uint32_t bits = 0;
+    // Pieces beyond the row are its last piece again (which changes no largest value), so that no branch keeps the pieces from
+    // being worked out side by side.
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      rows.template read<VEC>(min((int)threadIdx.x * VEC + i * stride, width - VEC), width, from, v[i]);
+      if (ROWS::GATED && VEC * ITEMS > 16) asm volatile("" ::: "memory");  // 32 units and their gates would not fit the registers
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (int)threadIdx.x * VEC + i * stride;
+      if (!ROWS::NORMED || c < width) {
+        if constexpr (ROWS::NORMED) {
+          float w[VEC];
+          rows.template ahead<VEC>(c, width, w);
+          rows.template settle<VEC, false>(row, c, width, w, v[i], squares);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) bits = max(bits, __float_as_uint(v[i][j]) & 0x7fffffffu);
+      }
+    }
+    meet<ROWS::NORMED>(bits, squares, most[side], sums[side]);
+    side ^= 1;
+    const bool given_up = *reinterpret_cast<volatile int*>(&abort_flag) != 0;
+    // every thread has its values: the stage is free for the row that comes so many turns later
+    if (threadIdx.x < 32) {
+      __syncwarp();
+      if (row + (long long)stages * gridDim.x < n && !given_up) fetch(row + stages * gridDim.x, s);
+    }
+    finish_row<ROWS, VEC, ITEMS>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
+    if (++s == stages) { s = 0; turn ^= 1; }
+    if (given_up) break;
   }
 }
 
@@ -280,8 +496,34 @@ template <typename TA, typename TW> bool fits(const NormedRows<TA, TW>& r, int w
   return pieces_fit(r.x, width, vec) && pieces_fit(r.weight, width, vec) && pieces_fit(r.add, width, vec) && pieces_fit(r.sum, width, vec);
 }
 
+template <class ROWS, int VEC, int PER>
+int launch_quantize_ring(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag,
+                         cudaStream_t stream, bool& taken) {
+  constexpr auto kernel = quantize_int8_ring_kernel<ROWS, VEC, PER / VEC>;
+  const int threads = ((width + PER - 1) / PER + 31) / 32 * 32, stage = ring_stage<ROWS>(width), room = 208 * 1024;
+  if (threads > ring_threads(PER)) return XRT_OK;
+  int blocks = ring_threads(PER) / threads < 8 ? ring_threads(PER) / threads : 8;
+  while (blocks > 1 && 2 * stage * blocks > room) --blocks;
+  int stages = room / blocks / stage;
+  if (stages > RING_MOST) stages = RING_MOST;
+  const int grid = blocks * multiprocessors();
+  taken = stages >= 2 && n > (ROWS::NORMED && VEC > 1 ? 8 : 1) * grid && stage >= RING_LEAST;
+  if (!taken) return XRT_OK;
+  const cudaError_t err = allow_shared_memory_once<kernel>(room);
+  if (err != cudaSuccess) return (int)err;
+  launch_kernel(kernel, dim3(grid), dim3(threads), (size_t)stages * stage, stream, codes, scales, rows, n, width, ld_codes, stages, error_flag);
+  return launch_status();
+}
+
 template <class ROWS, int VEC>
-int launch_quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, cudaStream_t stream) {
+int launch_quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag, cudaStream_t stream) {
+  bool taken = false;
+  int status = XRT_OK;
+  if (width <= 16 * 1024)
+    status = launch_quantize_ring<ROWS, VEC, 16>(codes, scales, rows, n, width, ld_codes, error_flag, stream, taken);
+  else if (width <= 32 * 1024)
+    status = launch_quantize_ring<ROWS, VEC, 32>(codes, scales, rows, n, width, ld_codes, error_flag, stream, taken);
+  if (taken || status != XRT_OK) return status;
   auto launch = [&](auto kernel, int per) {
     const int threads = per > 0 ? ((width + per - 1) / per + 31) / 32 * 32 : 1024;
     launch_kernel(kernel, dim3(n), dim3(threads), 0, stream, codes, scales, rows, width, ld_codes);
@@ -295,53 +537,55 @@ int launch_quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int w
 
 // Pieces of eight, four or one value at a time: the most that rows of this width and these addresses allow.
 template <class ROWS>
-int quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, cudaStream_t stream) {
+int quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag, cudaStream_t stream) {
   if (n < 0 || width <= 0 || ld_codes < width) return XRT_ERR_ARGUMENT;
   if (n == 0) return XRT_OK;
   auto whole = [&](int vec) {
     return width % vec == 0 && fits(rows, width, vec) && ((uintptr_t)codes | (uintptr_t)ld_codes) % vec == 0;
   };
-  if (whole(8)) return launch_quantize<ROWS, 8>(codes, scales, rows, n, width, ld_codes, stream);
-  if (whole(4)) return launch_quantize<ROWS, 4>(codes, scales, rows, n, width, ld_codes, stream);
-  return launch_quantize<ROWS, 1>(codes, scales, rows, n, width, ld_codes, stream);
+  if (whole(8)) return launch_quantize<ROWS, 8>(codes, scales, rows, n, width, ld_codes, error_flag, stream);
+  if (whole(4)) return launch_quantize<ROWS, 4>(codes, scales, rows, n, width, ld_codes, error_flag, stream);
+  return launch_quantize<ROWS, 1>(codes, scales, rows, n, width, ld_codes, error_flag, stream);
 }
 
 }  // namespace xrt
 
-// codes: int8 [n, width] with rows ld_codes bytes apart; scales: float32 [n].
+// codes: int8 [n, width] with rows ld_codes bytes apart; scales: float32 [n]; error_flag (may be null) is set to 7 if a bounded
+// wait ran out.
 
 // x [n, width], float32 or bfloat16.
 XRT_EXPORT int xrt_quantize_rows(void* codes, float* scales, const void* x, int n, int width, int ld_codes, int x_dtype,
-                                 cudaStream_t stream) {
+                                 int* error_flag, cudaStream_t stream) {
   XRT_DISPATCH_DTYPE(x_dtype, T, {
-    return xrt::quantize((int8_t*)codes, scales, xrt::PlainRows<T>{(const T*)x}, n, width, ld_codes, stream);
+    return xrt::quantize((int8_t*)codes, scales, xrt::PlainRows<T>{(const T*)x}, n, width, ld_codes, error_flag, stream);
   });
 }
 
 // gate_up [n, 2 * width], float32 or bfloat16; act and options as for xrt_swiglu.
 XRT_EXPORT int xrt_swiglu_int8(void* codes, float* scales, const void* gate_up, int n, int width, int ld_codes, int in_dtype,
-                               int act, const xrt::GateOptions* options, cudaStream_t stream) {
+                               int act, const xrt::GateOptions* options, int* error_flag, cudaStream_t stream) {
   if (act < 0 || act > 2) return XRT_ERR_ARGUMENT;
   xrt::RowScale gate;
   gate.gate_act = act;
   if (!xrt::take_gate_options(options, 2, width, gate)) return XRT_ERR_ARGUMENT;
   XRT_DISPATCH_DTYPE(in_dtype, T, {
-    return xrt::quantize((int8_t*)codes, scales, xrt::GatedRows<T>{(const T*)gate_up, gate}, n, width, ld_codes, stream);
+    return xrt::quantize((int8_t*)codes, scales, xrt::GatedRows<T>{(const T*)gate_up, gate}, n, width, ld_codes, error_flag, stream);
   });
 }
 
 // x float32 [n, width]; add (may be null) [n, width], float32 or bfloat16; with it sum [n, width] gets x + add (sum may be x).
 XRT_EXPORT int xrt_rmsnorm_int8(void* codes, float* scales, const float* x, const void* add, float* sum, const void* weight,
-                                int n, int width, int ld_codes, float eps, int add_dtype, int w_dtype, cudaStream_t stream) {
+                                int n, int width, int ld_codes, float eps, int add_dtype, int w_dtype, int* error_flag,
+                                cudaStream_t stream) {
   if (add != nullptr && sum == nullptr) return XRT_ERR_ARGUMENT;
   XRT_DISPATCH_DTYPE(w_dtype, TW, {
     if (add == nullptr) {
       const xrt::NormedRows<xrt::Nothing, TW> rows{x, nullptr, nullptr, (const TW*)weight, eps};
-      return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, stream);
+      return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, error_flag, stream);
     }
     XRT_DISPATCH_DTYPE(add_dtype, TA, {
       const xrt::NormedRows<TA, TW> rows{x, (const TA*)add, sum, (const TW*)weight, eps};
-      return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, stream);
+      return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, error_flag, stream);
     });
   });
 }

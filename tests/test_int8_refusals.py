@@ -56,3 +56,29 @@ def test_products():
     refused("float32", o.gemm_int8, out, codes, scales, w, w_scales, bias=torch.zeros(5, dtype=torch.bfloat16))
     too_long = o.INT8_MAX_INPUTS + 1
     refused("32 bits", o.gemm_int8, out, o.int8_rows(3, too_long, "cpu"), scales, o.int8_rows(5, too_long, "cpu"), w_scales)
+
+
+def test_models_that_hold_no_8_bit_weights():
+    from helpers import TINY_QWEN3
+    from xeno_rt_b200.config import config_from_dict
+    from xeno_rt_b200.core import ConfigError, Unsupported
+    from xeno_rt_b200.engine.model import check_weights_format
+    from zivovik_cases import CASE_MIXED as other
+
+    def spec(raw):
+        arch, config = config_from_dict(raw)
+        return arch.build_spec(config)
+
+    check_weights_format(spec(TINY_QWEN3), None)
+    check_weights_format(spec(TINY_QWEN3), "int8")
+    with pytest.raises(ConfigError, match="int4"):
+        check_weights_format(spec(TINY_QWEN3), "int4")
+    with pytest.raises(Unsupported, match="8-bit weights"):
+        check_weights_format(spec(other), "int8")
+
+
+def test_the_command_takes_the_option():
+    from xeno_rt_b200.cli import build_parser
+    args = build_parser().parse_args(["generate", "--model", "m", "--prompt-ids", "1", "--weights", "int8"])
+    assert args.weights == "int8"
+    assert build_parser().parse_args(["generate", "--model", "m", "--prompt-ids", "1"]).weights is None

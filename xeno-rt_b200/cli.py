@@ -5,7 +5,7 @@ generated ids go to standard output, the statistics line to standard error.
 
     python -m xeno_rt_b200 generate (--model DIR | --random-config CONFIG.json [--seed-weights N])
         --prompt-ids 1,2,3 [--prompt-ids 4,5 ...] [--max-tokens 128] [--temperature 0.8] [--top-k 40] [--top-p 0.95]
-        [--repetition-penalty 1.1] [--seed N] [--dtype bfloat16|float32] [--stop-ids 2,3] [--device cuda:0]
+        [--repetition-penalty 1.1] [--seed N] [--dtype bfloat16|float32] [--weights int8] [--stop-ids 2,3] [--device cuda:0]
 
 The reference's command takes its model from one of two sources, a file or a repository to fetch it
 from (main.rs:28-34); the two sources here are a folder (``--model``: config.json and safetensors,
@@ -45,6 +45,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--repetition-penalty", type=float, default=1.1)
     g.add_argument("--seed", type=int, default=None)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    g.add_argument("--weights", default=None, choices=["int8"],
+                   help="hold attention's and the feed-forwards' matrices in 8 bits (default: in --dtype)")
     g.add_argument("--stop-ids", type=_ids, default=None,
                    help="ids that end a sequence (default: eos_token_id of config.json)")
     g.add_argument("--device", default="cuda:0")
@@ -58,7 +60,7 @@ def run_generate(args) -> int:
     from .engine import GenerateRequest, Model, Runtime
 
     if args.model is not None:
-        runtime = Runtime.load(args.model, dtype=args.dtype, device=args.device)
+        runtime = Runtime.load(args.model, dtype=args.dtype, device=args.device, weights=args.weights)
     else:
         try:
             with open(args.random_config) as fh:
@@ -67,7 +69,8 @@ def run_generate(args) -> int:
             raise ConfigError(f"{args.random_config}: no such file") from None
         except json.JSONDecodeError as exc:
             raise ConfigError(f"{args.random_config}: not valid JSON ({exc})") from None
-        runtime = Runtime(Model.random(raw, seed=args.seed_weights, dtype=args.dtype, device=args.device))
+        runtime = Runtime(Model.random(raw, seed=args.seed_weights, dtype=args.dtype, device=args.device,
+                                       weights=args.weights))
     session = runtime.new_session()
     requests = [GenerateRequest(prompt_ids=p, max_tokens=args.max_tokens, temperature=args.temperature,
                                 top_k=args.top_k, top_p=args.top_p, repetition_penalty=args.repetition_penalty,

@@ -12,17 +12,36 @@ import torch
 
 from ..cache import Cache, KVNeed
 from ..config import config_from_dict, load_config
-from ..core import DType, KernelError, log, parse_dtype, torch_dtype
+from ..core import ConfigError, DType, KernelError, Unsupported, log, parse_dtype, torch_dtype
 from ..csrc import ops
 from ..parts import LayerParts, ModelSpec, part_class
 from ..weights import (INIT_MATRIX_STD, INIT_NORM_STD, load_weights, tensor_key)
 from ..weights.loader import LoadedTensors, kept_dtype, locate_tensors
 
 
+def check_weights_format(spec: ModelSpec, weights: str | None) -> None:
+    """Raises where a model's weights cannot be held as asked: "int8" is for layers of a norm, attention, a norm and a gated
+    feed-forward, as the Llama and Qwen3 decoders have."""
+    if weights is None:
+        return
+    if weights != "int8":
+        raise ConfigError(f"weights {weights!r} is not None or 'int8'")
+    for i, layer in enumerate(spec.layers):
+        kinds = {name: part.kind for name, (_, part) in layer.parts.items()}
+        if layer.arrangement != "prenorm_residual" or kinds != {"mixer_norm": "rmsnorm", "mixer": "attention",
+                                                                "ffn_norm": "rmsnorm", "ffn": "swiglu"}:
+            raise Unsupported(f"layer {i} ({layer.arrangement}: {', '.join(kinds.values())}): 8-bit weights are for pre-norm layers "
+                              f"of attention and a gated feed-forward")
+
+
 class Model:
-    def __init__(self, spec: ModelSpec, tensors: dict, dtype: DType, device, config=None):
+    def __init__(self, spec: ModelSpec, tensors: dict, dtype: DType, device, config=None, weights: str | None = None):
+        """``weights`` = "int8": the matrices of attention and feed-forwards are held in 8 bits with a scale a row, and their
+        products run on 8-bit integers (parts/int8.py); ``tensors`` then gives each up once it has been laid out."""
         ops.require_device()
         spec.validate()
+        check_weights_format(spec, weights)
+        self.weights_format = weights
         self.spec = spec
         self.config = config
         self.dtype = dtype
@@ -41,7 +60,14 @@ class Model:
                 buffer = shared.get(tuple(part_spec.weights[r] for r in roles))
                 if buffer is not None:  # the loader put these tensors side by side already
                     weights[fused_role] = buffer
-            return cls(part_spec.params, weights, dtype, self.device)
+            part = cls(part_spec.params, weights, dtype, self.device)
+            if self.weights_format == "int8" and hasattr(part, "use_int8"):
+                part.use_int8()
+                for name in part_spec.weights.values():  # the stored form of its matrices is needed no more
+                    tensors.pop(name)
+                for names in [n for n in shared if set(n) <= set(part_spec.weights.values())]:
+                    shared.pop(names)
+            return part
 
         self.embedding = build("embedding", spec.embedding)
         self.stream_parts = {name: build("stream", part) for name, part in spec.stream_parts.items()}
@@ -69,9 +95,9 @@ class Model:
 
     # ------------------------------------------------------------------ construction
     @classmethod
-    def load(cls, folder: str, dtype="bfloat16", device="cuda:0") -> "Model":
+    def load(cls, folder: str, dtype="bfloat16", device="cuda:0", weights: str | None = None) -> "Model":
         """From a folder with config.json and model.safetensors; the model class is chosen by
-        config.json's architecture name."""
+        config.json's architecture name.  ``weights``: None, or "int8" (see ``__init__``)."""
         ops.require_device()
         dtype = parse_dtype(dtype)
         arch, config = load_config(folder)
@@ -79,21 +105,23 @@ class Model:
             header = locate_tensors(folder)[0]
             config = config.with_tensor_shapes({name: tuple(meta["shape"]) for name, meta in header.items()})
         spec = arch.build_spec(config)
+        check_weights_format(spec, weights)
         tensors = load_weights(folder, spec.expected_tensors(), dtype, device, spec.ignorable_tensors,
                                fused_groups=spec.fused_groups())
         log("info", f"loaded {arch.name} from {folder}: {len(spec.layers)} layers, width {spec.hidden_size}, "
-                    f"vocabulary {spec.vocab_size}, {dtype.label}")
-        return cls(spec, tensors, dtype, device, config)
+                    f"vocabulary {spec.vocab_size}, {dtype.label}{', 8-bit weights' if weights else ''}")
+        return cls(spec, tensors, dtype, device, config, weights)
 
     @classmethod
-    def random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0") -> "Model":
+    def random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", weights: str | None = None) -> "Model":
         """Random weights drawn on the device from ``seed`` with the generator of
-        weights/random_init.py, without a model folder (for models of many gigabytes)."""
+        weights/random_init.py, without a model folder (for models of many gigabytes).  ``weights`` as for ``load``."""
         ops.require_device()
         dtype = parse_dtype(dtype)
         raw = config if isinstance(config, dict) else config.to_dict()
         arch, typed = config_from_dict(raw)
         spec = arch.build_spec(typed)
+        check_weights_format(spec, weights)
         tensors = LoadedTensors()
         expected = {e.name: e for e in spec.expected_tensors()}
         for group in spec.fused_groups():  # one buffer for tensors that a part wants side by side
@@ -114,7 +142,7 @@ class Model:
             else:
                 ops.fill_normal(t, tensor_key(seed, e.name), 0.0, INIT_MATRIX_STD)
             tensors[e.name] = t
-        return cls(spec, tensors, dtype, device, typed)
+        return cls(spec, tensors, dtype, device, typed, weights)
 
     # ------------------------------------------------------------------ cache
     def _layer_needs(self, layer: LayerParts) -> dict:

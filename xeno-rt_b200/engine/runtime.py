@@ -107,8 +107,9 @@ class Runtime:
 
     @classmethod
     def load(cls, path: str, dtype="bfloat16", device="cuda:0", cache_tokens: int | None = None,
-             max_batch: int = 64) -> "Runtime":
-        return cls(Model.load(path, dtype=dtype, device=device), cache_tokens, max_batch)
+             max_batch: int = 64, weights: str | None = None) -> "Runtime":
+        """``weights`` = "int8": attention's and the feed-forwards' matrices in 8 bits (``Model``)."""
+        return cls(Model.load(path, dtype=dtype, device=device, weights=weights), cache_tokens, max_batch)
 
     def new_session(self) -> "Session":
         return Session(self)

@@ -14,6 +14,7 @@ import torch
 from ..cache import KVNeed, StateNeed
 from ..core import ConfigError, DType, Unsupported, torch_dtype
 from ..csrc import ops
+from .int8 import Int8Matrix
 from .linear import linear
 from .registry import part_class, register_part
 
@@ -85,6 +86,7 @@ class GroupedQueryAttention:
     and meet zero columns, so the result is that of the true sizes."""
 
     graph_safe = True
+    takes_int8 = False  # whether the input may be ``Int8Rows`` (see ``use_int8``)
 
     @classmethod
     def _sizes(cls, params):
@@ -256,6 +258,12 @@ class GroupedQueryAttention:
         self.dtype = dtype
         self.act_dtype = torch_dtype(dtype)
 
+    def use_int8(self) -> None:
+        """Holds the matrices of the products in 8 bits from here on; their inputs are rounded to 8 bits too."""
+        self.w_qkv, self.w_o = Int8Matrix.of(self.w_qkv), Int8Matrix.of(self.w_o)
+        self.w_q = self.w_qkv[: self.q_width]
+        self.takes_int8 = True
+
     def cache_need(self):
         # a chunk's keys are among as many most recent ones: what lies behind those can be given back
         bounds = [int(b) for b in (self.window, self.chunk) if b]
@@ -266,7 +274,7 @@ class GroupedQueryAttention:
 
     def takes_pending_norm(self, rows: int, device) -> bool:
         """Whether the first product of ``forward`` can finish a norm that the part before prepared."""
-        if self.dtype is not DType.BF16:
+        if self.dtype is not DType.BF16 or self.takes_int8:
             return False
         from . import linear_bf16
         return linear_bf16.takes_pending(rows, self.w_qkv.shape[0], self.width, "store", device)

@@ -43,15 +43,22 @@ def prenorm_residual(parts: LayerParts, x, ctx, stores, owns_cache: bool) -> Non
     maps a part's name to the cache storage it asked for."""
     h = ctx.take_pending(parts.mixer_norm)  # the layer before may have prepared this layer's first norm
     if h is None:
-        h = parts.mixer_norm.forward(x)
+        h = _normed(parts.mixer_norm, parts.mixer, x)
     ctx.then_norm = _norm_that_can_wait(parts.ffn_norm, parts.ffn, ctx, x)
     parts.mixer.forward(h, x, ctx, stores.get("mixer"), owns_cache)
     h = ctx.take_pending(parts.ffn_norm)
     if h is None:
-        h = parts.ffn_norm.forward(x)
+        h = _normed(parts.ffn_norm, parts.ffn, x)
     after = ctx.shared.get("next_layer")  # (norm, the part that takes its result) of the layer that runs next
     ctx.then_norm = _norm_that_can_wait(after[0], after[1], ctx, x) if after else None
     parts.ffn.forward(h, x, ctx)
+
+
+def _normed(norm, consumer, x):
+    """The norm of the stream as the part that takes it wants it: in 8 bits where it says so and the norm can."""
+    if getattr(consumer, "takes_int8", False) and hasattr(norm, "forward_int8"):
+        return norm.forward_int8(x)
+    return norm.forward(x)
 
 
 def _norm_that_can_wait(norm, consumer, ctx, x):

@@ -7,6 +7,7 @@ import torch
 
 from ..core import ConfigError, DType, torch_dtype
 from ..csrc import ops
+from .int8 import Int8Matrix, Int8Rows
 from .linear import linear
 from .norm import WeightedParts
 from .registry import register_part
@@ -21,6 +22,7 @@ class SwiGLUFeedForward:
     ``down_bias`` [width]."""
 
     graph_safe = True
+    takes_int8 = False  # whether the input may be ``Int8Rows`` (see ``use_int8``)
 
     @classmethod
     def fused_weights(cls, params):
@@ -55,14 +57,25 @@ class SwiGLUFeedForward:
         if self.activation == "gated_sigmoid" and not (self.gate.limit > 0 and self.gate.alpha > 0):
             raise ConfigError("a limited gate needs a positive limit and alpha")
 
+    def use_int8(self) -> None:
+        """Holds the matrices of the products in 8 bits from here on; their inputs are rounded to 8 bits too."""
+        self.w_gate_up, self.w_down = Int8Matrix.of(self.w_gate_up), Int8Matrix.of(self.w_down)
+        self.takes_int8 = True
+
     def takes_pending_norm(self, rows: int, device) -> bool:
         """Whether the first product of ``forward`` can finish a norm that the part before prepared."""
-        if self.act_dtype != torch.bfloat16 or self.activation != "silu" or self.gate.bias is not None:
+        if self.takes_int8 or self.act_dtype != torch.bfloat16 or self.activation != "silu" or self.gate.bias is not None:
             return False
         from . import linear_bf16
         return linear_bf16.takes_pending(rows, self.inner, self.width, "swiglu", device)
 
     def _act(self, h):
+        if self.takes_int8:
+            # the gate's and the up rows' sums in the compute dtype: half the bytes of 32 bits, and 8 bits are kept
+            both = linear(h, self.w_gate_up, out_dtype=self.act_dtype)
+            act = Int8Rows(h.shape[0], self.inner, h.device)
+            ops.swiglu_int8(act.codes, act.scales, both, self.gate)
+            return act
         act = torch.empty((h.shape[0], self.inner), dtype=self.act_dtype, device=h.device)
         fused = False
         if self.act_dtype == torch.bfloat16 and h.dtype == torch.bfloat16:

@@ -6,6 +6,8 @@ import torch
 
 from ..core import KernelError
 from ..csrc import ops
+from .int8 import Int8Matrix
+from .int8 import product as int8_product
 
 
 def linear(x, weight: torch.Tensor, out_dtype=None, accumulate_into: torch.Tensor | None = None, then_norm=None,
@@ -15,7 +17,8 @@ def linear(x, weight: torch.Tensor, out_dtype=None, accumulate_into: torch.Tenso
     Accumulation is 32-bit in every kernel.  ``x`` may be a ``PendingNorm`` (see parts/norm.py).
     ``then_norm`` (an RMSNorm part, with ``accumulate_into``): if the kernel that runs can prepare that
     norm of the new residual on its way, the result is (residual, PendingNorm), else (residual, None).
-    ``out`` (a contiguous tensor [M, N]): the product is written there instead of into a new tensor."""
+    ``out`` (a contiguous tensor [M, N]): the product is written there instead of into a new tensor.
+    ``weight`` may be an ``Int8Matrix`` and ``x`` then ``Int8Rows`` too (see parts/int8.py)."""
     if out is not None and (accumulate_into is not None or tuple(out.shape) != (x.shape[0], weight.shape[0])
                             or not out.is_contiguous()):
         raise KernelError("linear: out must be a contiguous [rows, weight rows] tensor, and not given with accumulate_into")
@@ -38,7 +41,10 @@ def linear(x, weight: torch.Tensor, out_dtype=None, accumulate_into: torch.Tenso
     pending = None
     if m > 0:
         done = False
-        if weight.dtype == torch.bfloat16 and x.dtype == torch.bfloat16:
+        if isinstance(weight, Int8Matrix):
+            int8_product(out, x, weight, accumulate)
+            done = True
+        elif weight.dtype == torch.bfloat16 and x.dtype == torch.bfloat16:
             from . import linear_bf16
             if accumulate and then_norm is not None:
                 pending = linear_bf16.run_with_norm(out, x, weight, then_norm)

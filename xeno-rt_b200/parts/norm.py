@@ -8,6 +8,7 @@ import torch
 
 from ..core import ConfigError, torch_dtype
 from ..csrc import ops
+from .int8 import Int8Rows
 from .registry import register_part
 
 
@@ -81,6 +82,12 @@ class RMSNorm:
         n = x.shape[0] if rows is None else rows.numel()
         out = torch.empty((n, self.width), dtype=self.out_dtype, device=x.device)
         ops.rmsnorm(out, x, self.weight, self.eps, rows)
+        return out
+
+    def forward_int8(self, x):
+        """The norm of the rows ``x`` as ``Int8Rows``, for products of 8-bit integers."""
+        out = Int8Rows(x.shape[0], self.width, x.device)
+        ops.rmsnorm_int8(out.codes, out.scales, x, self.weight, self.eps)
         return out
 
     def forward_f32(self, x):

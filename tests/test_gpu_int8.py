@@ -67,6 +67,18 @@ def test_ties_go_to_even_and_the_largest_is_127():
     assert codes[0].tolist() == [127, -127, 0, 2, 2, 0, -2, -2, 126, 126]
 
 
+@pytest.mark.parametrize("rows,width", [(3, 100), (5, 4096), (600, 4096), (500, 8191), (3, 40000)])
+def test_rows_are_divided_as_32_bit_numbers_are(rows, width):
+    """Of 16-bit values, whose quotients often lie in the middle: the codes of x / scale, rounded, then to even."""
+    x = (normal(rows, width, seed=80) * 8).round().to(torch.bfloat16)  # few values, many ties
+    codes, scales, _ = room(rows, width)
+    ops().quantize_rows(codes, scales, x)
+    x = x.float().cpu().numpy()  # (numpy divides; torch multiplies by the inverse of a number)
+    scale = np.maximum(np.abs(x).max(axis=1) / np.float32(127), np.float32(TINY))
+    assert scale.dtype == np.float32 and np.array_equal(scales.cpu().numpy(), scale)
+    assert np.array_equal(codes.cpu().numpy(), np.rint(x / scale[:, None]))
+
+
 @pytest.mark.parametrize("rows", [1, 3, 700])
 @pytest.mark.parametrize("width", [33, 512])
 def test_rows_whose_addresses_allow_only_single_values(rows, width):
@@ -78,7 +90,7 @@ def test_rows_whose_addresses_allow_only_single_values(rows, width):
 
 
 # more rows than blocks: rows that come through a ring, at every 16-byte phase, with rows that begin and end anywhere
-MANY = [(3000, 33), (1500, 1600), (1300, 3001), (700, 4096), (1203, 4099), (333, 8190), (150, 14337), (400, 16384), (450, 25600),
+MANY = [(700, 4100), (450, 8204), (150, 25604), (3000, 33), (1500, 1600), (1300, 3001), (700, 4096), (1203, 4099), (333, 8190), (150, 14337), (400, 16384), (450, 25600),
         (449, 25001), (301, 26000), (300, 30000), (152, 33000)]
 
 
@@ -97,7 +109,7 @@ def test_many_rows(rows, width, dtype):
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
-@pytest.mark.parametrize("rows,width", [(1203, 1999), (700, 4096), (333, 7005), (301, 14336), (160, 12800), (155, 12801)])
+@pytest.mark.parametrize("rows,width", [(1203, 1999), (900, 2052), (700, 4096), (620, 4100), (333, 7005), (301, 14336), (160, 12800), (155, 12801), (151, 20004)])
 def test_many_gates(rows, width, act, dtype):
     gate_up = (normal(rows, 2 * width, seed=71) * 3).to(DT[dtype])
     codes, scales, whole = room(rows, width)
@@ -106,7 +118,8 @@ def test_many_gates(rows, width, act, dtype):
 
 
 @pytest.mark.parametrize("add", [None, "float32", "bfloat16"])
-@pytest.mark.parametrize("rows,width", [(1203, 1999), (1000, 2048), (700, 4096), (613, 4099), (333, 8190), (300, 13000), (170, 20001)])
+@pytest.mark.parametrize("rows,width", [(1203, 1999), (9000, 1028), (5000, 2052), (6000, 2048), (4000, 4096), (3700, 4100), (613, 4099), (333, 8190), (1400, 13000),
+                                        (170, 20001)])
 def test_many_norms(rows, width, add):
     x = normal(rows, width, seed=72)
     w = 1 + 0.1 * normal(width, seed=73)
@@ -391,6 +404,25 @@ def test_two_products_at_once():
     for want, got in zip(alone, outs):
         for out in got:
             assert torch.equal(out, want)
+
+
+def test_weights_that_the_call_before_wrote():
+    """A norm and a product whose weights were made right before them, without ``constant_weight``."""
+    o = ops()
+    x = normal(4, 4096, seed=90)
+    w = [normal(4096, 4096, seed=91 + i) for i in range(4)]
+    ones = torch.ones(4096, device=DEV)
+    want = [o_rows(one) for one in w]
+    held, held_scales = o.int8_rows(4096, 4096, DEV), torch.empty(4096, device=DEV)
+    h, h_scales = o.int8_rows(4, 4096, DEV), torch.empty(4, device=DEV)
+    o.rmsnorm_int8(h, h_scales, x, ones, 1e-5)
+    outs = [torch.empty(4, 4096, device=DEV) for _ in w]
+    torch.cuda.synchronize()
+    for one, out in zip(w, outs):
+        o.quantize_rows(held, held_scales, one)
+        o.gemm_int8(out, h, h_scales, held, held_scales)
+    for (codes, scales), out in zip(want, outs):
+        check_product(out, *product(h, h_scales, codes, scales))
 
 
 def test_empty_calls():

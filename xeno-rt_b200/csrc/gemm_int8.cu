@@ -16,6 +16,8 @@
 //               bytes are stored by the warp, a row of 32 columns at a time.
 // Every wait on an mbarrier is bounded.  A wait that runs out raises the error flag and an abort flag in shared memory; all
 // roles leave their loops, the block frees its TMEM and returns.
+#include <stddef.h>
+
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -756,23 +758,37 @@ int launch_gemm_int8_few(const Int8Product& p, int constant_weight, cudaStream_t
 
 }  // namespace xrt
 
-// codes: int8 [M, K] with rows ldx bytes apart; w: int8 [N, K] with rows ldw bytes apart; both strides multiples of 16 and both
-// bases 16-byte aligned; scales float32 [M], w_scales float32 [N], bias float32 [N] or null.  out: [M, N] with row
-// stride ldo; mode 0 stores, 1 adds into a float32 out.  constant_weight: none of the kernels that may still run wrote w, which
-// is then read ahead of the wait for them.  error_flag (may be null) is set to 6 if a bounded wait ran out.
-XRT_EXPORT int xrt_gemm_int8(void* out, const void* codes, const float* scales, const void* w, const float* w_scales,
-                             const float* bias, int M, int N, int K, int ldx, int ldw, int ldo, int out_dtype, int mode,
-                             int constant_weight, int* error_flag, cudaStream_t stream) {
-  if (M < 0 || N <= 0 || K <= 0 || K > 131071 || ldx < K || ldw < K || ldo < N || mode < 0 || mode > 1) return XRT_ERR_ARGUMENT;
-  if (mode == 1 && out_dtype != XRT_F32) return XRT_ERR_ARGUMENT;
-  if (ldx % 16 != 0 || ldw % 16 != 0 || ((uintptr_t)codes & 15) || ((uintptr_t)w & 15)) return XRT_ERR_UNSUPPORTED;
-  if (M == 0) return XRT_OK;
-  const xrt::Int8Product p{out, codes, w, M, N, K, ldx, ldw, ldo, {scales, w_scales, bias}, xrt::multiprocessors(), error_flag};
+// A call as the caller packs it.  codes: int8 [M, K] with rows ldx bytes apart; w: int8 [N, K] with rows ldw bytes apart; both
+// strides multiples of 16 and both bases 16-byte aligned; scales float32 [M], w_scales float32 [N], bias float32 [N] or null.
+// out: [M, N] with row stride ldo; mode 0 stores, 1 adds into a float32 out.  constant_weight: none of the kernels that may
+// still run wrote w, which is then read ahead of the wait for them.  error_flag (may be null) is set to 6 if a bounded wait
+// ran out.
+struct XrtInt8Call {
+  void* out;
+  const void* codes;
+  const float* scales;
+  const void* w;
+  const float* w_scales;
+  const float* bias;
+  int* error_flag;
+  int M, N, K, ldx, ldw, ldo, out_dtype, mode, constant_weight;
+};
+static_assert(offsetof(XrtInt8Call, M) == 56 && offsetof(XrtInt8Call, constant_weight) == 88, "seven pointers, then nine ints");
+
+XRT_EXPORT int xrt_gemm_int8(const XrtInt8Call* call, cudaStream_t stream) {
+  const XrtInt8Call& c = *call;
+  if (c.M < 0 || c.N <= 0 || c.K <= 0 || c.K > 131071 || c.ldx < c.K || c.ldw < c.K || c.ldo < c.N || c.mode < 0 || c.mode > 1)
+    return XRT_ERR_ARGUMENT;
+  if (c.mode == 1 && c.out_dtype != XRT_F32) return XRT_ERR_ARGUMENT;
+  if (c.ldx % 16 != 0 || c.ldw % 16 != 0 || ((uintptr_t)c.codes & 15) || ((uintptr_t)c.w & 15)) return XRT_ERR_UNSUPPORTED;
+  if (c.M == 0) return XRT_OK;
+  const xrt::Int8Product p{c.out, c.codes, c.w, c.M, c.N, c.K, c.ldx, c.ldw, c.ldo, {c.scales, c.w_scales, c.bias},
+                           xrt::multiprocessors(), c.error_flag};
   if (p.sm_count <= 1) return XRT_ERR_UNSUPPORTED;
-  const bool few = M <= xrt::FEW_MAX_ROWS;
-  if (mode == 1)
-    return few ? xrt::launch_gemm_int8_few<1, float>(p, constant_weight, stream) : xrt::launch_gemm_int8<1, float>(p, stream);
-  XRT_DISPATCH_DTYPE(out_dtype, TO, {
-    return few ? xrt::launch_gemm_int8_few<0, TO>(p, constant_weight, stream) : xrt::launch_gemm_int8<0, TO>(p, stream);
+  const bool few = c.M <= xrt::FEW_MAX_ROWS;
+  if (c.mode == 1)
+    return few ? xrt::launch_gemm_int8_few<1, float>(p, c.constant_weight, stream) : xrt::launch_gemm_int8<1, float>(p, stream);
+  XRT_DISPATCH_DTYPE(c.out_dtype, TO, {
+    return few ? xrt::launch_gemm_int8_few<0, TO>(p, c.constant_weight, stream) : xrt::launch_gemm_int8<0, TO>(p, stream);
   });
 }

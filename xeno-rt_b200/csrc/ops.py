@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import dataclasses
+import struct
 import threading
 
 import torch
@@ -93,8 +94,8 @@ _SIGNATURES = {
     "xrt_recurrence_step": [_P, _P, _P, _P, _P, _P, _I, _P],
     "xrt_quantize_rows": [_P, _P, _P, _I, _I, _I, _I, _P, _P],
     "xrt_swiglu_int8": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P],
-    "xrt_rmsnorm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _P, _P],
-    "xrt_gemm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "xrt_rmsnorm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _P, _P],
+    "xrt_gemm_int8": [_P, _P],
     "xrt_fill_normal": [_P, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_double, _I, _P],
     "xrt_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P],
     "xrt_mark_seen": [_P, _I, _P, _P, _I, _I, _P],
@@ -1705,24 +1706,26 @@ def int8_rows(rows: int, width: int, device) -> torch.Tensor:
 
 
 # A launch of a few microseconds should not wait for its checks: the raw handle of a device's current stream and the current
-# device's number cost a tenth of a microsecond each, ``torch.cuda.current_stream`` two.
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
+# device's number cost a tenth of a microsecond each, ``torch.cuda.current_stream`` two; and seventeen arguments packed into
+# one structure half of one, as arguments of a foreign call two.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_pack_int8_product = struct.Struct("7Q9i").pack
 
 
-def _run_int8(what: str, tensors, function: str, args) -> None:
+def _run_int8(what: str, tensors, launcher, args) -> None:
     """Calls a launcher on the one device that all of ``tensors`` (None: not given) lie on, whichever is current, and on
     that device's current stream."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and (t.get_device() != index or index < 0):
             raise KernelError(f"{what}: all tensors must be on one CUDA device")
-    launcher = getattr(_lib or library(), function)
-    if index == torch.cuda.current_device():
-        _check(launcher(*args, _raw_stream(index)), what)
+    if index == _current_device():
+        status = launcher(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            _check(launcher(*args, _raw_stream(index)), what)
+            status = launcher(*args, _raw_stream(index))
+    _check(status, what)
 
 
 def _error_flag_pointer(index: int) -> int:
@@ -1740,8 +1743,8 @@ def _codes(t, name: str, what: str, rows: int, width: int) -> int:
     if t.dtype != torch.int8 or t.shape != (rows, width):
         raise KernelError(f"{what}: {name} must be int8 [{rows}, {width}], not {t.dtype} {tuple(t.shape)}")
     distance, step = t.stride()
-    if (width > 1 and step != 1) or (rows > 1 and distance < width):
-        raise KernelError(f"{what}: the rows of {name} must be contiguous")
+    if (width > 1 and step != 1) or (rows > 1 and not width <= distance < 1 << 31):
+        raise KernelError(f"{what}: the rows of {name} must be contiguous and less than 2^31 bytes apart")
     return distance if rows > 1 else -(-width // 16) * 16
 
 
@@ -1763,7 +1766,7 @@ def quantize_rows(codes, scales, x) -> None:
     ld = _codes(codes, "codes", what, n, width)
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), n, width, ld, _code(x.dtype),
             _error_flag_pointer(x.get_device()))
-    _run_int8(what, (x, codes, scales), "xrt_quantize_rows", args)
+    _run_int8(what, (x, codes, scales), _kernels().xrt_quantize_rows, args)
 
 
 def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
@@ -1780,14 +1783,15 @@ def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
     options = gate.options(width)
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), n, width, ld, _code(gate_up.dtype),
             code, options, _error_flag_pointer(gate_up.get_device()))
-    _run_int8(what, (gate_up, codes, scales, gate.bias), "xrt_swiglu_int8", args)
+    _run_int8(what, (gate_up, codes, scales, gate.bias), _kernels().xrt_swiglu_int8, args)
 
 
-def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None) -> None:
+def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None, constant_weight: bool = False) -> None:
     """The RMSNorm of the residual stream as 8-bit integers, something added to the stream on the way: s = x + add (``add``
     float32 or bfloat16 [n, width], or None: s = x), written to ``out`` (float32 [n, width]; None: into ``x``); codes[r],
     scales[r] are ``quantize_rows`` of s[r] / sqrt(mean(s[r]^2) + eps) * weight, which is 32-bit and not written.  ``x``
-    float32 [n, width], ``weight`` float32 or bfloat16 [width]."""
+    float32 [n, width], ``weight`` float32 or bfloat16 [width].  ``constant_weight``: the weight is a model's, which no kernel
+    that may still run has written: it is then read while the kernel before finishes."""
     what = "rmsnorm_int8"
     if x.dim() != 2 or tuple(weight.shape) != (x.shape[1],):
         raise KernelError(f"{what}: x must be [rows, width] and weight [width]")
@@ -1801,8 +1805,9 @@ def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None) -> No
     ld = _codes(codes, "codes", what, n, width)
     args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),
             _ptr(out, "out", torch.float32), _ptr(weight, "weight"), n, width, ld, float(eps),
-            0 if add is None else _code(add.dtype), _code(weight.dtype), _error_flag_pointer(x.get_device()))
-    _run_int8(what, (x, codes, scales, weight, add, out), "xrt_rmsnorm_int8", args)
+            0 if add is None else _code(add.dtype), _code(weight.dtype), 1 if constant_weight else 0,
+            _error_flag_pointer(x.get_device()))
+    _run_int8(what, (x, codes, scales, weight, add, out), _kernels().xrt_rmsnorm_int8, args)
 
 
 def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = False, bias=None,
@@ -1814,25 +1819,28 @@ def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = Fals
     weight is a model's, which no kernel that may still run has written: products of few rows then read it while the
     kernel before them finishes."""
     what = "gemm_int8"
-    if codes.dim() != 2 or weight.dim() != 2 or codes.shape[1] != weight.shape[1]:
-        raise KernelError(f"{what}: shapes do not fit: codes {tuple(codes.shape)}, weight {tuple(weight.shape)}")
+    if codes.dim() != 2 or weight.dim() != 2:
+        raise KernelError(f"{what}: codes and weight must be [rows, inputs]")
     m, k = codes.shape
-    n = weight.shape[0]
+    n, inputs = weight.shape
+    if k != inputs:
+        raise KernelError(f"{what}: shapes do not fit: codes {tuple(codes.shape)}, weight {tuple(weight.shape)}")
     if k > INT8_MAX_INPUTS:
         raise KernelError(f"{what}: sums over {k} inputs can pass 32 bits; at most {INT8_MAX_INPUTS} are taken")
     ldx, ldw = _codes(codes, "codes", what, m, k), _codes(weight, "weight", what, n, k)
-    if (ldx | ldw | codes.data_ptr() | weight.data_ptr()) % 16:
-        name = "codes" if (ldx | codes.data_ptr()) % 16 else "weight"
+    at, weight_at = codes.data_ptr(), weight.data_ptr()
+    if (ldx | ldw | at | weight_at) % 16:
+        name = "codes" if (ldx | at) % 16 else "weight"
         raise KernelError(f"{what}: the rows of {name} must begin every so many 16 bytes (see int8_rows)")
     if out.shape != (m, n):
         raise KernelError(f"{what}: out must be [{m}, {n}], not {tuple(out.shape)}")
-    out_distance, step = out.stride()
-    if (n > 1 and step != 1) or (m > 1 and out_distance < n):
-        raise KernelError(f"{what}: the rows of out must be contiguous")
+    ldo, step = out.stride()
+    if (n > 1 and step != 1) or (m > 1 and not n <= ldo < 1 << 31):
+        raise KernelError(f"{what}: the rows of out must be contiguous and less than 2^31 elements apart")
     if accumulate and out.dtype != torch.float32:
         raise KernelError(f"{what}: only a float32 out is added into")
-    args = (out.data_ptr(), codes.data_ptr(), _vector(scales, "scales", what, m), weight.data_ptr(),
-            _vector(weight_scales, "weight_scales", what, n), 0 if bias is None else _vector(bias, "bias", what, n), m, n, k,
-            ldx, ldw, out_distance if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0,
-            _error_flag_pointer(out.get_device()))
-    _run_int8(what, (out, codes, scales, weight, weight_scales, bias), "xrt_gemm_int8", args)
+    call = _pack_int8_product(
+        out.data_ptr(), at, _vector(scales, "scales", what, m), weight_at, _vector(weight_scales, "weight_scales", what, n),
+        0 if bias is None else _vector(bias, "bias", what, n), _error_flag_pointer(out.get_device()), m, n, k, ldx, ldw,
+        ldo if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0)
+    _run_int8(what, (out, codes, scales, weight, weight_scales, bias), _kernels().xrt_gemm_int8, (call,))

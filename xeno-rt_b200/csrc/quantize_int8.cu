@@ -64,12 +64,22 @@ __device__ __forceinline__ void store_some(float* p, const float (&v)[VEC]) {
   }
 }
 
-// The codes of VEC values y * inverse; all zero with `broken`.
-template <int VEC>
-__device__ __forceinline__ void store_codes(int8_t* p, const float (&y)[VEC], float inverse, bool broken) {
+// The codes of VEC values y / scale, `inverse` being 1 / scale; all zero with `broken`.  EXACT: of the quotient as a 32-bit division
+// rounds it (the product with the inverse, corrected once by its remainder).  A row that is coded as it is needs that: its values
+// have few bits, and quotients in the middle between two codes, which go to the even one, are many.  What was computed on
+// the way here is not exact in its last bit.
+template <int VEC, bool EXACT>
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&y)[VEC], float scale, float inverse, bool broken) {
   uint32_t bits[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) bits[i] = __float_as_uint(fmaf(y[i], inverse, ROUNDER));
+  for (int i = 0; i < VEC; ++i) {
+    if constexpr (EXACT) {
+      const float q = y[i] * inverse;
+      bits[i] = __float_as_uint(fmaf(fmaf(-q, scale, y[i]), inverse, q) + ROUNDER);
+    } else {
+      bits[i] = __float_as_uint(fmaf(y[i], inverse, ROUNDER));
+    }
+  }
   if constexpr (VEC == 1) {
     *p = broken ? 0 : (int8_t)(bits[0] & 0xff);
   } else {
@@ -90,12 +100,13 @@ __device__ __forceinline__ void store_codes(int8_t* p, const float (&y)[VEC], fl
 template <typename T>
 struct PlainRows {
   static constexpr bool NORMED = false;
-  static constexpr bool GATED = false;
+  static constexpr bool GATED = false, EXACT = true;
   static constexpr int STREAMS = 1;  // what a row consists of in memory: pieces of `length` elements of From<i>
   template <int I> using From = T;
   const T* x;
   template <int I> __host__ __device__ __forceinline__ const T* from() const { return x; }
   __host__ __device__ __forceinline__ static int length(int width) { return width; }
+  static constexpr int early = 0;
   __device__ __forceinline__ void wait() { pdl_wait(x); }
   // the values from a row's streams where those lie in shared memory
   template <int VEC, class READ> __device__ __forceinline__ void read(int c, int, const READ& get, float (&v)[VEC]) const { get.template operator()<0, VEC>(c, v); }
@@ -110,13 +121,14 @@ struct PlainRows {
 template <typename T>
 struct GatedRows {
   static constexpr bool NORMED = false;
-  static constexpr bool GATED = true;
+  static constexpr bool GATED = true, EXACT = false;
   static constexpr int STREAMS = 1;
   template <int I> using From = T;
   const T* gate_up;  // [rows, 2 * width]
   RowScale gate;
   template <int I> __host__ __device__ __forceinline__ const T* from() const { return gate_up; }
   __host__ __device__ __forceinline__ static int length(int width) { return 2 * width; }
+  static constexpr int early = 0;
   __device__ __forceinline__ void wait() { pdl_wait(gate_up); }
   template <int VEC> __device__ __forceinline__ void gated(float (&v)[VEC], float (&u)[VEC], int c) const {
     // the fast exponential and division, as for a bfloat16 result: 8 bits are kept
@@ -156,7 +168,7 @@ template <typename TA, typename TW>
 struct NormedRows {
   static constexpr bool NORMED = true;
   static constexpr bool ADDS = !std::is_same<TA, Nothing>::value;
-  static constexpr bool GATED = false;
+  static constexpr bool GATED = false, EXACT = false;
   static constexpr int STREAMS = ADDS ? 2 : 1;
   template <int I> using From = std::conditional_t<I == 0, float, TA>;
   template <int I> __host__ __device__ __forceinline__ const From<I>* from() const {
@@ -178,8 +190,8 @@ struct NormedRows {
   float* sum;  // may be x
   const TW* weight;
   float eps;
+  int early;  // the weight may be read before the kernel before this one is done
   __device__ __forceinline__ void wait() { pdl_wait(x, add); }
-  // the weight does not depend on the step: it is on its way before the wait for the kernel before
   template <int VEC> __device__ __forceinline__ void ahead(int c, int width, float (&w)[VEC]) const {
     if (c < width) load_some<VEC>(weight + c, w);
   }
@@ -254,7 +266,7 @@ __device__ __forceinline__ void finish_row(int8_t* codes, float* scales, const R
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[i][j] *= s.factor;
       }
-      store_codes<VEC>(dst + c, v[i], s.inverse, s.broken);
+      store_codes<VEC, ROWS::EXACT>(dst + c, v[i], s.scale, s.inverse, s.broken);
     }
   }
 }
@@ -270,11 +282,13 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
   pdl_trigger();
   float w[KEPT][VEC], v[KEPT][VEC];
   const int stride = (int)blockDim.x * VEC;
-  if constexpr (AHEAD) {
+  const bool waited = !rows.early;
+  if (waited) rows.wait();
+  if constexpr (AHEAD) {  // a model's weight is on its way before the wait for the kernel before
 #pragma unroll
     for (int i = 0; i < KEPT; ++i) rows.template ahead<VEC>((int)threadIdx.x * VEC + i * stride, width, w[i]);
   }
-  rows.wait();
+  if (!waited) rows.wait();
   const int row = blockIdx.x;
   float squares = 0.f;
   uint32_t bits = 0;
@@ -320,7 +334,7 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[0][j] *= s.factor;
       }
-      store_codes<VEC>(dst + c, v[0], s.inverse, s.broken);
+      store_codes<VEC, ROWS::EXACT>(dst + c, v[0], s.scale, s.inverse, s.broken);
     }
   }
 }
@@ -414,7 +428,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
   auto fetch = [&](int row, int s) {  // the first warp
     unsigned char* place = ring + s * stage_bytes;
     const uint32_t bar = smem_u32(&full[s]);
-    if constexpr (VEC == 1) {  // (else rows begin and end at 16-byte boundaries)
+    if constexpr (VEC < 8) {  // (else rows begin and end at 16-byte boundaries)
       ring_edges<ROWS, 0>(rows, row, width, place, lane);
       if constexpr (ROWS::STREAMS == 2) ring_edges<ROWS, 1>(rows, row, width, place + room0, lane);
       __syncwarp();
@@ -441,7 +455,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
     }
     const unsigned char* place = ring + s * stage_bytes;
     RingRow<ROWS> from{place, place + room0};
-    if constexpr (VEC == 1) {
+    if constexpr (VEC < 8) {
       from.first += (uintptr_t)ring_source<ROWS, 0>(rows, row, width) & 15;
       if constexpr (ROWS::STREAMS == 2) from.second += (uintptr_t)ring_source<ROWS, 1>(rows, row, width) & 15;
     }
@@ -573,18 +587,19 @@ XRT_EXPORT int xrt_swiglu_int8(void* codes, float* scales, const void* gate_up, 
   });
 }
 
+// constant_weight: none of the kernels that may still run wrote the weight.
 // x float32 [n, width]; add (may be null) [n, width], float32 or bfloat16; with it sum [n, width] gets x + add (sum may be x).
 XRT_EXPORT int xrt_rmsnorm_int8(void* codes, float* scales, const float* x, const void* add, float* sum, const void* weight,
-                                int n, int width, int ld_codes, float eps, int add_dtype, int w_dtype, int* error_flag,
-                                cudaStream_t stream) {
+                                int n, int width, int ld_codes, float eps, int add_dtype, int w_dtype, int constant_weight,
+                                int* error_flag, cudaStream_t stream) {
   if (add != nullptr && sum == nullptr) return XRT_ERR_ARGUMENT;
   XRT_DISPATCH_DTYPE(w_dtype, TW, {
     if (add == nullptr) {
-      const xrt::NormedRows<xrt::Nothing, TW> rows{x, nullptr, nullptr, (const TW*)weight, eps};
+      const xrt::NormedRows<xrt::Nothing, TW> rows{x, nullptr, nullptr, (const TW*)weight, eps, constant_weight};
       return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, error_flag, stream);
     }
     XRT_DISPATCH_DTYPE(add_dtype, TA, {
-      const xrt::NormedRows<TA, TW> rows{x, (const TA*)add, sum, (const TW*)weight, eps};
+      const xrt::NormedRows<TA, TW> rows{x, (const TA*)add, sum, (const TW*)weight, eps, constant_weight};
       return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, error_flag, stream);
     });
   });

@@ -87,7 +87,7 @@ class RMSNorm:
     def forward_int8(self, x):
         """The norm of the rows ``x`` as ``Int8Rows``, for products of 8-bit integers."""
         out = Int8Rows(x.shape[0], self.width, x.device)
-        ops.rmsnorm_int8(out.codes, out.scales, x, self.weight, self.eps)
+        ops.rmsnorm_int8(out.codes, out.scales, x, self.weight, self.eps, constant_weight=True)
         return out
 
     def forward_f32(self, x):

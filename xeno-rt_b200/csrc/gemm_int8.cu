@@ -137,6 +137,11 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       const bool codes = warp == 0;
       const CUtensorMap* map = codes ? &map_x : &map_w;
       asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+      if (!codes) {  // the first of W on its way to the L2 while the kernel before finishes
+        int m_blk, n_blk;
+        int8_tile_place<TILE_ROWS>(unit, tiles_m, tiles_n, m_blk, n_blk);
+        for (int kb = 0; kb < min(STAGES, k_iters); ++kb) tma_prefetch_2d(map, kb * I8_BK, n_blk * BN + rank * Shape::B_ROWS);
+      }
       pdl_wait();
       const uint32_t stages = smem_u32(codes ? a_stages : b_stages), bytes = codes ? Shape::A_BYTES : Shape::B_ROWS * I8_BK;
       int s = 0;
@@ -396,7 +401,7 @@ int launch_gemm_int8(const Int8Product& p, cudaStream_t stream) {
 // kernel this short also pays for every instruction that it meets for the first time (its code comes from the L2): the
 // finish is one short loop, and while warps 5-8 wait they walk it once into a place that nobody reads.
 constexpr int FEW_MAX_ROWS = 128, FEW_MAX_SPLITS = 4, FEW_MAX_STAGES = 24;
-constexpr int FEW_PRODUCERS = 4;
+constexpr int FEW_PRODUCERS = 4;  // (the walk below counts on four)
 constexpr int FEW_THREADS = 32 * (FEW_PRODUCERS + 1 + 4);
 constexpr int FEW_TAIL_BYTES = 512 + 4 * (FEW_MAX_ROWS + 2 * 256);  // barriers, flags, a place that nobody reads; scales, biases
 
@@ -407,7 +412,8 @@ struct FewShape {
   int splits;
   int slabs;     // of 128 of K in a stage: 1, 2 or 4
   int stages;
-  int k_iters;   // stages' worth of K
+  int k_iters;   // stages' worth of K: the first `k_more` parts have k_each + 1, the others k_each
+  int k_each, k_more;
   int early;     // the weight may be read before the kernel before this one is done
 };
 
@@ -451,8 +457,9 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   pdl_trigger();
   if (splits > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = (int)blockIdx.x / splits, split = (int)blockIdx.x - tile * splits;
-  const int kb0 = shape.k_iters * split / splits, kb1 = shape.k_iters * (split + 1) / splits;
+  // (nothing here divides: what a block does before its first copies is a tenth of a short product)
+  const int tile = (int)blockIdx.y, split = (int)blockIdx.x;
+  const int kb0 = shape.k_each * split + min(split, shape.k_more), kb1 = kb0 + shape.k_each + (split < shape.k_more ? 1 : 0);
   const int groups = shape.rows > 128 ? 2 : 1;
   int tmem_cols = 32;
   while (tmem_cols < groups * nb) tmem_cols *= 2;
@@ -477,7 +484,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       // rows of codes that belong to it.  Neighbouring tiles start their walk over K at different places: blocks that run at the
       // same time would else ask for the same lines of the codes, and for addresses a whole weight row apart, at the same moment.
       const uint64_t once = policy_evict_first();
-      const int count = kb1 - kb0, first = tile * 5 % count;
+      const int count = kb1 - kb0, first = (tile * 5 & 15) * count >> 4;
       const int units = count * slabs, ahead = min(stages, count) * slabs;
       const int w_load = shape.rows * I8_BK;
       struct Walk {
@@ -485,15 +492,15 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       };
       auto begin = [&]() {
         Walk at;
-        at.s = warp / slabs;
-        at.i = warp % slabs;
+        at.s = slabs == 1 ? warp : slabs == 2 ? warp >> 1 : 0;
+        at.i = warp & (slabs - 1);
         at.k = first + at.s;
         while (at.s >= stages) at.s -= stages;
         while (at.k >= count) at.k -= count;
         return at;
       };
       auto step = [&](Walk& at) {  // four slabs further
-        const int on = FEW_PRODUCERS / slabs;
+        const int on = slabs == 1 ? 4 : slabs == 2 ? 2 : 1;
         at.s += on;
         while (at.s >= stages) at.s -= stages;
         at.k += on;
@@ -508,7 +515,12 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                     ((kb0 + at.k) * slabs + at.i) * I8_BK, 0, smem_u32(&full[at.s]));
       };
       Walk at = begin();
-      if (!shape.early) pdl_wait();
+      if (!shape.early) {  // into the L2 at least (more than the ring was slower: 8 rows of 4,096, 14,336 12.7 -> 13.5 us)
+        for (int u = warp; u < ahead; u += FEW_PRODUCERS, step(at))
+          tma_prefetch_2d(&map_w, ((kb0 + at.k) * slabs + at.i) * I8_BK, tile * shape.rows);
+        at = begin();
+        pdl_wait();
+      }
       for (int u = warp; u < ahead; u += FEW_PRODUCERS, step(at)) {
         mbar_expect_tx(smem_u32(&full[at.s]), w_load);
         load_w(at);
@@ -580,7 +592,11 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     asm volatile("bar.sync 1, 128;" ::: "memory");
   }
   const int row_lo = split * per, n_lo = tile * shape.rows + row_lo;
-  const int here = max(0, min(min(per, shape.rows - row_lo), shape.N - n_lo)), quads = (shape.M + 3) / 4;
+  const int here = max(1, min(min(per, shape.rows - row_lo), shape.N - n_lo));
+  const int eights = n_lo < shape.N && row_lo < shape.rows ? (shape.M + 7) / 8 : 0;
+  // this thread's first sums, and from some to the next: eight rows of codes, weight rows inside
+  const int eight0 = (int)threadIdx.x / here, local0 = (int)threadIdx.x - eight0 * here;
+  const int eight_step = FEW_THREADS / here, local_step = FEW_THREADS - eight_step * here;
 #pragma unroll 1
   for (int pass = warp > FEW_PRODUCERS ? 0 : 1; pass < 2; ++pass) {
     if (pass == 1) {
@@ -616,34 +632,39 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       else __syncthreads();
       if (*abort_flag) break;
     }
-    const int begin = pass == 1 ? (int)threadIdx.x : 0, end = pass == 1 ? here * quads : 1, wide = max(here, 1);
+    int eight = pass == 1 ? eight0 : 0, local = pass == 1 ? local0 : 0;
 #pragma unroll 1
-    for (int idx = begin; idx < end; idx += FEW_THREADS) {
-      const int quad = idx / wide, local = idx - quad * wide;
-      int sums[4] = {0, 0, 0, 0};
+    while (eight < (pass == 1 ? eights : 1)) {
+      int sums[8] = {};
 #pragma unroll 1
       for (int sp = 0; sp < splits; ++sp) {
-        const int4 part = *reinterpret_cast<const int4*>(recv + (sp * per + local) * recv_row + quad * 4);
-        sums[0] += part.x; sums[1] += part.y; sums[2] += part.z; sums[3] += part.w;
+        const int4* part = reinterpret_cast<const int4*>(recv + (sp * per + local) * recv_row + eight * 8);
+        const int4 lo = part[0], hi = part[1];
+        sums[0] += lo.x; sums[1] += lo.y; sums[2] += lo.z; sums[3] += lo.w;
+        sums[4] += hi.x; sums[5] += hi.y; sums[6] += hi.z; sums[7] += hi.w;
       }
-      const float4 by_row = *reinterpret_cast<const float4*>(row_scales + quad * 4);
+      const float4 s_lo = *reinterpret_cast<const float4*>(row_scales + eight * 8), s_hi = *reinterpret_cast<const float4*>(row_scales + eight * 8 + 4);
       const float by_column = column_scales[row_lo + local], bias = biases[row_lo + local];
-      const float factors[4] = {by_row.x, by_row.y, by_row.z, by_row.w};
+      const float factors[8] = {s_lo.x, s_lo.y, s_lo.z, s_lo.w, s_hi.x, s_hi.y, s_hi.z, s_hi.w};
       // rows beyond M, and all rows of the first walk, go nowhere; what is added into is asked for before the first store,
       // which might be to the same memory
-      TO* dst[4];
-      float old[4];
+      TO* dst[8];
+      float old[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = quad * 4 + e;
+      for (int e = 0; e < 8; ++e) {
+        const int m = eight * 8 + e;
         dst[e] = pass == 1 && m < shape.M ? out + (size_t)m * shape.ldo + n_lo + local : reinterpret_cast<TO*>(nowhere);
         old[e] = MODE == 1 ? to_float(*dst[e]) : 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const float value = fmaf(__int2float_rn(sums[e]) * factors[e], by_column, bias);
         *dst[e] = from_float<TO>(MODE == 1 ? old[e] + value : value);
       }
+      if (pass == 0) break;
+      eight += eight_step;
+      local += local_step;
+      if (local >= here) { local -= here; ++eight; }
     }
   }
   __syncthreads();
@@ -738,7 +759,9 @@ int launch_gemm_int8_few(const Int8Product& p, int constant_weight, cudaStream_t
   if (!make_map_int8_2d(&map_x, p.codes, p.M, p.K, p.ldx, shape.nb) || !make_map_int8_2d(&map_w, p.w, p.N, p.K, p.ldw, shape.rows))
     return XRT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)((shape.N + shape.rows - 1) / shape.rows) * shape.splits);
+  shape.k_each = shape.k_iters / shape.splits;
+  shape.k_more = shape.k_iters - shape.k_each * shape.splits;
+  config.gridDim = dim3((unsigned)shape.splits, (unsigned)((shape.N + shape.rows - 1) / shape.rows));
   config.blockDim = dim3(FEW_THREADS);
   config.dynamicSmemBytes = few_shared_bytes(shape);
   config.stream = stream;
@@ -785,7 +808,7 @@ XRT_EXPORT int xrt_gemm_int8(const XrtInt8Call* call, cudaStream_t stream) {
   const xrt::Int8Product p{c.out, c.codes, c.w, c.M, c.N, c.K, c.ldx, c.ldw, c.ldo, {c.scales, c.w_scales, c.bias},
                            xrt::multiprocessors(), c.error_flag};
   if (p.sm_count <= 1) return XRT_ERR_UNSUPPORTED;
-  const bool few = c.M <= xrt::FEW_MAX_ROWS;
+  const bool few = c.M <= xrt::FEW_MAX_ROWS && c.N <= 65535 * 64;  // (tiles, of 64 rows at least, are a grid's second dimension)
   if (c.mode == 1)
     return few ? xrt::launch_gemm_int8_few<1, float>(p, c.constant_weight, stream) : xrt::launch_gemm_int8<1, float>(p, stream);
   XRT_DISPATCH_DTYPE(c.out_dtype, TO, {

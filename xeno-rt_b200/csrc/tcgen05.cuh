@@ -88,6 +88,12 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
                ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar), "l"(policy) : "memory");
 }
 
+// The same tile into the L2 only.  A line that is written after it was fetched there is written there: unlike a load, this may
+// come before the wait for a kernel that might still write the tile.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
+
 // Two blocks as one (cta_group::2): the pair is a cluster of two, block 0 of it issues the MMAs, and both blocks' copies
 // complete on block 0's barriers.
 __device__ __forceinline__ void cluster_sync() {

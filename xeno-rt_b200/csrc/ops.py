@@ -92,9 +92,9 @@ _SIGNATURES = {
     "xrt_recurrence_gates": [_P, _P, _P, _P, _P, _I, _P],
     "xrt_recurrence_scan": [_P, _P, _I, _I, _P],
     "xrt_recurrence_step": [_P, _P, _P, _P, _P, _P, _I, _P],
-    "xrt_quantize_rows": [_P, _P, _P, _I, _I, _I, _I, _P, _P],
-    "xrt_swiglu_int8": [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P],
-    "xrt_rmsnorm_int8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _P, _P],
+    "xrt_quantize_rows": [_P, _P],
+    "xrt_swiglu_int8": [_P, _P],
+    "xrt_rmsnorm_int8": [_P, _P],
     "xrt_gemm_int8": [_P, _P],
     "xrt_fill_normal": [_P, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_double, _I, _P],
     "xrt_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P],
@@ -1707,24 +1707,25 @@ def int8_rows(rows: int, width: int, device) -> torch.Tensor:
 
 # A launch of a few microseconds should not wait for its checks: the raw handle of a device's current stream and the current
 # device's number cost a tenth of a microsecond each, ``torch.cuda.current_stream`` two; and seventeen arguments packed into
-# one structure half of one, as arguments of a foreign call two.
+# one structure a half, as arguments of a foreign call two.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _pack_int8_product = struct.Struct("7Q9i").pack
+_pack_int8_rows = struct.Struct("8Q8if").pack
 
 
-def _run_int8(what: str, tensors, launcher, args) -> None:
-    """Calls a launcher on the one device that all of ``tensors`` (None: not given) lie on, whichever is current, and on
-    that device's current stream."""
+def _run_int8(what: str, tensors, launcher, call) -> None:
+    """Makes a packed call of a launcher on the one device that all of ``tensors`` (None: not given) lie on, whichever is
+    current, and on that device's current stream."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and (t.get_device() != index or index < 0):
             raise KernelError(f"{what}: all tensors must be on one CUDA device")
     if index == _current_device():
-        status = launcher(*args, _raw_stream(index))
+        status = launcher(call, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = launcher(*args, _raw_stream(index))
+            status = launcher(call, _raw_stream(index))
     _check(status, what)
 
 
@@ -1764,9 +1765,9 @@ def quantize_rows(codes, scales, x) -> None:
         raise KernelError(f"{what}: x must be [rows, width]")
     n, width = x.shape
     ld = _codes(codes, "codes", what, n, width)
-    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), n, width, ld, _code(x.dtype),
-            _error_flag_pointer(x.get_device()))
-    _run_int8(what, (x, codes, scales), _kernels().xrt_quantize_rows, args)
+    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), 0, 0, 0, 0,
+                           _error_flag_pointer(x.get_device()), n, width, ld, _code(x.dtype), 0, 0, 0, 0, 0.0)
+    _run_int8(what, (x, codes, scales), _kernels().xrt_quantize_rows, call)
 
 
 def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
@@ -1780,10 +1781,11 @@ def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
         raise KernelError(f"{what}: gate_up must be [rows, 2 * width]")
     n, width = gate_up.shape[0], gate_up.shape[1] // 2
     ld = _codes(codes, "codes", what, n, width)
-    options = gate.options(width)
-    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), n, width, ld, _code(gate_up.dtype),
-            code, options, _error_flag_pointer(gate_up.get_device()))
-    _run_int8(what, (gate_up, codes, scales, gate.bias), _kernels().xrt_swiglu_int8, args)
+    options = gate.options(width)  # (a reference, which the call needs alive)
+    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), 0, 0, 0,
+                           0 if options is None else ctypes.addressof(options._obj), _error_flag_pointer(gate_up.get_device()),
+                           n, width, ld, _code(gate_up.dtype), 0, 0, code, 0, 0.0)
+    _run_int8(what, (gate_up, codes, scales, gate.bias), _kernels().xrt_swiglu_int8, call)
 
 
 def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None, constant_weight: bool = False) -> None:
@@ -1803,11 +1805,11 @@ def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None, const
         if add.shape != x.shape or out.shape != x.shape:
             raise KernelError(f"{what}: add and out must have the shape of x")
     ld = _codes(codes, "codes", what, n, width)
-    args = (codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),
-            _ptr(out, "out", torch.float32), _ptr(weight, "weight"), n, width, ld, float(eps),
-            0 if add is None else _code(add.dtype), _code(weight.dtype), 1 if constant_weight else 0,
-            _error_flag_pointer(x.get_device()))
-    _run_int8(what, (x, codes, scales, weight, add, out), _kernels().xrt_rmsnorm_int8, args)
+    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),
+                           _ptr(out, "out", torch.float32), _ptr(weight, "weight"), 0, _error_flag_pointer(x.get_device()),
+                           n, width, ld, 0, 0 if add is None else _code(add.dtype), _code(weight.dtype), 0,
+                           1 if constant_weight else 0, eps)
+    _run_int8(what, (x, codes, scales, weight, add, out), _kernels().xrt_rmsnorm_int8, call)
 
 
 def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = False, bias=None,
@@ -1843,4 +1845,4 @@ def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = Fals
         out.data_ptr(), at, _vector(scales, "scales", what, m), weight_at, _vector(weight_scales, "weight_scales", what, n),
         0 if bias is None else _vector(bias, "bias", what, n), _error_flag_pointer(out.get_device()), m, n, k, ldx, ldw,
         ldo if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0)
-    _run_int8(what, (out, codes, scales, weight, weight_scales, bias), _kernels().xrt_gemm_int8, (call,))
+    _run_int8(what, (out, codes, scales, weight, weight_scales, bias), _kernels().xrt_gemm_int8, call)

@@ -6,13 +6,15 @@
 // A row of zeros has codes 0 and the smallest scale.  A row with a NaN or an infinity has codes 0 and the scale NaN, so that
 // every product with it is NaN.  Sums, statistics and y are 32-bit; the codes are the only rounding to fewer bits.
 //
-// One block a row, the row in registers: read once, one meeting of the block (the norm's sum of squares and the largest |s w| are found in the same pass, since the factor 1 / rms is the
-// same for the whole row), codes written once.  The largest absolute value is found on the bits: for numbers without
+// One block a row, the row in registers: read once, one meeting of the block (the norm's sum of squares and the largest |s w|
+// are found in the same pass, since the factor 1 / rms is the same for the whole row), codes written once.  The largest absolute value is found on the bits: for numbers without
 // a sign their order is that of the integers, and every NaN lies above infinity.
 //
 // Few rows (steps): a block a row, its loads all in flight together.  More rows than blocks: blocks take every so many-th
 // row from a ring in shared memory that bulk copies fill ahead (quantize_int8_ring_kernel), so that the memory is asked for the
 // next rows while a block meets.  Rows beyond what 1,024 threads hold are walked twice.
+#include <stddef.h>
+
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -564,43 +566,55 @@ int quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int width, i
 
 }  // namespace xrt
 
-// codes: int8 [n, width] with rows ld_codes bytes apart; scales: float32 [n]; error_flag (may be null) is set to 7 if a bounded
-// wait ran out.
+// A call as the caller packs it.  codes: int8 [n, width] with rows ld_codes bytes apart; scales: float32 [n]; error_flag (may be
+// null) is set to 7 if a bounded wait ran out.
+struct XrtRowsCall {
+  void* codes;
+  float* scales;
+  const void* x;
+  const void* add;
+  float* sum;
+  const void* weight;
+  const xrt::GateOptions* gate;
+  int* error_flag;
+  int n, width, ld_codes, x_dtype, add_dtype, w_dtype, act, constant_weight;
+  float eps;
+};
+static_assert(offsetof(XrtRowsCall, n) == 64 && offsetof(XrtRowsCall, eps) == 96, "eight pointers, eight ints, a float");
+
+template <class ROWS>
+static int quantize_call(const XrtRowsCall& c, const ROWS& rows, cudaStream_t stream) {
+  return xrt::quantize((int8_t*)c.codes, c.scales, rows, c.n, c.width, c.ld_codes, c.error_flag, stream);
+}
 
 // x [n, width], float32 or bfloat16.
-XRT_EXPORT int xrt_quantize_rows(void* codes, float* scales, const void* x, int n, int width, int ld_codes, int x_dtype,
-                                 int* error_flag, cudaStream_t stream) {
-  XRT_DISPATCH_DTYPE(x_dtype, T, {
-    return xrt::quantize((int8_t*)codes, scales, xrt::PlainRows<T>{(const T*)x}, n, width, ld_codes, error_flag, stream);
-  });
+XRT_EXPORT int xrt_quantize_rows(const XrtRowsCall* call, cudaStream_t stream) {
+  const XrtRowsCall& c = *call;
+  XRT_DISPATCH_DTYPE(c.x_dtype, T, { return quantize_call(c, xrt::PlainRows<T>{(const T*)c.x}, stream); });
 }
 
-// gate_up [n, 2 * width], float32 or bfloat16; act and options as for xrt_swiglu.
-XRT_EXPORT int xrt_swiglu_int8(void* codes, float* scales, const void* gate_up, int n, int width, int ld_codes, int in_dtype,
-                               int act, const xrt::GateOptions* options, int* error_flag, cudaStream_t stream) {
-  if (act < 0 || act > 2) return XRT_ERR_ARGUMENT;
+// x: gate_up [n, 2 * width], float32 or bfloat16; act and gate as for xrt_swiglu.
+XRT_EXPORT int xrt_swiglu_int8(const XrtRowsCall* call, cudaStream_t stream) {
+  const XrtRowsCall& c = *call;
+  if (c.act < 0 || c.act > 2) return XRT_ERR_ARGUMENT;
   xrt::RowScale gate;
-  gate.gate_act = act;
-  if (!xrt::take_gate_options(options, 2, width, gate)) return XRT_ERR_ARGUMENT;
-  XRT_DISPATCH_DTYPE(in_dtype, T, {
-    return xrt::quantize((int8_t*)codes, scales, xrt::GatedRows<T>{(const T*)gate_up, gate}, n, width, ld_codes, error_flag, stream);
-  });
+  gate.gate_act = c.act;
+  if (!xrt::take_gate_options(c.gate, 2, c.width, gate)) return XRT_ERR_ARGUMENT;
+  XRT_DISPATCH_DTYPE(c.x_dtype, T, { return quantize_call(c, xrt::GatedRows<T>{(const T*)c.x, gate}, stream); });
 }
 
-// constant_weight: none of the kernels that may still run wrote the weight.
 // x float32 [n, width]; add (may be null) [n, width], float32 or bfloat16; with it sum [n, width] gets x + add (sum may be x).
-XRT_EXPORT int xrt_rmsnorm_int8(void* codes, float* scales, const float* x, const void* add, float* sum, const void* weight,
-                                int n, int width, int ld_codes, float eps, int add_dtype, int w_dtype, int constant_weight,
-                                int* error_flag, cudaStream_t stream) {
-  if (add != nullptr && sum == nullptr) return XRT_ERR_ARGUMENT;
-  XRT_DISPATCH_DTYPE(w_dtype, TW, {
-    if (add == nullptr) {
-      const xrt::NormedRows<xrt::Nothing, TW> rows{x, nullptr, nullptr, (const TW*)weight, eps, constant_weight};
-      return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, error_flag, stream);
-    }
-    XRT_DISPATCH_DTYPE(add_dtype, TA, {
-      const xrt::NormedRows<TA, TW> rows{x, (const TA*)add, sum, (const TW*)weight, eps, constant_weight};
-      return xrt::quantize((int8_t*)codes, scales, rows, n, width, ld_codes, error_flag, stream);
+// constant_weight: none of the kernels that may still run wrote the weight.
+XRT_EXPORT int xrt_rmsnorm_int8(const XrtRowsCall* call, cudaStream_t stream) {
+  const XrtRowsCall& c = *call;
+  if (c.add != nullptr && c.sum == nullptr) return XRT_ERR_ARGUMENT;
+  const float* x = (const float*)c.x;
+  XRT_DISPATCH_DTYPE(c.w_dtype, TW, {
+    const TW* weight = (const TW*)c.weight;
+    if (c.add == nullptr)
+      return quantize_call(c, xrt::NormedRows<xrt::Nothing, TW>{x, nullptr, nullptr, weight, c.eps, c.constant_weight}, stream);
+    XRT_DISPATCH_DTYPE(c.add_dtype, TA, {
+      return quantize_call(c, xrt::NormedRows<TA, TW>{x, (const TA*)c.add, c.sum, weight, c.eps, c.constant_weight}, stream);
     });
   });
 }

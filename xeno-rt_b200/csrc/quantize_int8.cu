@@ -24,6 +24,43 @@ namespace xrt {
 constexpr float CODE_MAX = 127.0f, SMALLEST_SCALE = 1.17549435e-38f;
 constexpr float ROUNDER = 12582912.0f;  // 1.5 * 2^23: v + ROUNDER has v, rounded to a whole number, in its low bits
 
+// Two 32-bit numbers in one instruction: a row's arithmetic is bound by the instructions that a multiprocessor can issue.
+struct Two {
+  uint64_t bits;
+  Two() = default;
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+
+// The largest absolute value of a row's pieces; a NaN once any is one.
+template <int VEC>
+__device__ __forceinline__ float largest_of(float most, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(most) : "f"(most), "f"(fabsf(v[0])));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2)
+      asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(most) : "f"(most), "f"(fabsf(v[i])), "f"(fabsf(v[i + 1])));
+  }
+  return most;
+}
+
 template <int VEC>
 __device__ __forceinline__ void load_some(const float* p, float (&v)[VEC]) {
   if constexpr (VEC % 4 == 0) {
@@ -73,13 +110,26 @@ __device__ __forceinline__ void store_some(float* p, const float (&v)[VEC]) {
 template <int VEC, bool EXACT>
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&y)[VEC], float scale, float inverse, bool broken) {
   uint32_t bits[VEC];
+  if constexpr (VEC == 1) {
+    float q = y[0] * inverse;
+    if constexpr (EXACT) q = fmaf(fmaf(-q, scale, y[0]), inverse, q) + ROUNDER;
+    else q = fmaf(y[0], inverse, ROUNDER);
+    bits[0] = __float_as_uint(q);
+  } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    if constexpr (EXACT) {
-      const float q = y[i] * inverse;
-      bits[i] = __float_as_uint(fmaf(fmaf(-q, scale, y[i]), inverse, q) + ROUNDER);
-    } else {
-      bits[i] = __float_as_uint(fmaf(y[i], inverse, ROUNDER));
+    for (int i = 0; i < VEC; i += 2) {
+      const Two both(y[i], y[i + 1]);
+      Two code;
+      if constexpr (EXACT) {
+        const Two q = both * Two(inverse);
+        code = fma_two(fma_two(q, Two(-scale), both), Two(inverse), q) + Two(ROUNDER);
+      } else {
+        code = fma_two(both, Two(inverse), Two(ROUNDER));
+      }
+      float first, second;
+      code.get(first, second);
+      bits[i] = __float_as_uint(first);
+      bits[i + 1] = __float_as_uint(second);
     }
   }
   if constexpr (VEC == 1) {
@@ -124,6 +174,7 @@ template <typename T>
 struct GatedRows {
   static constexpr bool NORMED = false;
   static constexpr bool GATED = true, EXACT = false;
+  static constexpr float GELU = 1.5957691216057308f;  // 2 sqrt(2 / pi)
   static constexpr int STREAMS = 1;
   template <int I> using From = T;
   const T* gate_up;  // [rows, 2 * width]
@@ -132,17 +183,40 @@ struct GatedRows {
   __host__ __device__ __forceinline__ static int length(int width) { return 2 * width; }
   static constexpr int early = 0;
   __device__ __forceinline__ void wait() { pdl_wait(gate_up); }
-  template <int VEC> __device__ __forceinline__ void gated(float (&v)[VEC], float (&u)[VEC], int c) const {
-    // the fast exponential and division, as for a bfloat16 result: 8 bits are kept
-    if (gate.gate_act == 1) {
-      // 0.5 g (1 + tanh(z)) = g sigmoid(2 z), which loses nothing where tanh(z) is near -1: alone in its row, such a
-      // value is the scale
-      add_gate_biases<VEC, true>(v, u, c, gate);
+  // g sigmoid(a g) u as g / (1 + 2^(-a log2(e) g)) u, with the exponent -a log2(e) g given: the exponential and the reciprocal
+  // as the multiprocessor has them (2 ulp and 1; 8 bits are kept), which end at 0 and infinity as the formula does.
+  __device__ __forceinline__ static float sigmoid(float exponent) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(exponent));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+  }
+  template <int VEC> __device__ __forceinline__ void gated(float (&g)[VEC], float (&u)[VEC], int c) const {
+    constexpr float LOG2E = 1.4426950408889634f;
+    add_gate_biases<VEC, true>(g, u, c, gate);
+    if (gate.gate_act == 2) {
+      const float limit = gate.gate_limit, exponent = -gate.gate_alpha * LOG2E;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        v[i] = swish_for<__nv_bfloat16>(v[i], 1.5957691216057308f * fmaf(0.044715f * v[i], v[i], 1.0f)) * u[i];
+      for (int i = 0; i < VEC; ++i) {
+        const float x = fminf(g[i], limit);
+        g[i] = x * sigmoid(x * exponent) * (fminf(fmaxf(u[i], -limit), limit) + 1.0f);
+      }
+      return;
+    }
+    // 0.5 g (1 + tanh(z)) = g sigmoid(2 z), which loses nothing where tanh(z) is near -1: alone in its row, such a
+    // value is the scale
+    const bool tanh_form = gate.gate_act == 1;
+    if constexpr (VEC == 1) {
+      g[0] = g[0] * sigmoid(g[0] * (tanh_form ? fmaf(-GELU * 0.044715f * LOG2E, g[0] * g[0], -GELU * LOG2E) : -LOG2E)) * u[0];
     } else {
-      gated_units<__nv_bfloat16, VEC, true>(v, u, c, gate);
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) {
+        const Two x(g[i], g[i + 1]);
+        const Two exponent = x * (tanh_form ? fma_two(x * x, Two(-GELU * 0.044715f * LOG2E), Two(-GELU * LOG2E)) : Two(-LOG2E));
+        float first, second;
+        exponent.get(first, second);
+        (x * Two(sigmoid(first), sigmoid(second)) * Two(u[i], u[i + 1])).get(g[i], g[i + 1]);
+      }
     }
   }
   template <int VEC, class READ> __device__ __forceinline__ void read(int c, int width, const READ& get, float (&v)[VEC]) const {
@@ -292,8 +366,7 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
   }
   if (!waited) rows.wait();
   const int row = blockIdx.x;
-  float squares = 0.f;
-  uint32_t bits = 0;
+  float squares = 0.f, most_here = 0.f;
   if constexpr (ITEMS > 0) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -308,8 +381,7 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
       if (c < width) {
         if constexpr (!AHEAD) rows.template ahead<VEC>(c, width, w[i]);
         rows.template settle<VEC, false>(row, c, width, w[i], v[i], squares);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) bits = max(bits, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        most_here = largest_of<VEC>(most_here, v[i]);
       }
     }
   } else {
@@ -317,10 +389,10 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
       rows.template ahead<VEC>(c, width, w[0]);
       rows.template load<VEC, false>(row, c, width, v[0]);
       rows.template settle<VEC, false>(row, c, width, w[0], v[0], squares);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) bits = max(bits, __float_as_uint(v[0][j]) & 0x7fffffffu);
+      most_here = largest_of<VEC>(most_here, v[0]);
     }
   }
+  uint32_t bits = __float_as_uint(most_here);
   meet<ROWS::NORMED>(bits, squares, most, sums);
   if constexpr (ITEMS > 0) {
     finish_row<ROWS, VEC, KEPT>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
@@ -461,8 +533,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
       from.first += (uintptr_t)ring_source<ROWS, 0>(rows, row, width) & 15;
       if constexpr (ROWS::STREAMS == 2) from.second += (uintptr_t)ring_source<ROWS, 1>(rows, row, width) & 15;
     }
-    float v[ITEMS][VEC], squares = 0.f;
-    uint32_t bits = 0;
+    float v[ITEMS][VEC], squares = 0.f, most_here = 0.f;
     // Pieces beyond the row are its last piece again (which changes no largest value), so that no branch keeps the pieces from
     // being worked out side by side.
 #pragma unroll
@@ -479,10 +550,10 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
           rows.template ahead<VEC>(c, width, w);
           rows.template settle<VEC, false>(row, c, width, w, v[i], squares);
         }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) bits = max(bits, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        most_here = largest_of<VEC>(most_here, v[i]);
       }
     }
+    uint32_t bits = __float_as_uint(most_here);
     meet<ROWS::NORMED>(bits, squares, most[side], sums[side]);
     side ^= 1;
     const bool given_up = *reinterpret_cast<volatile int*>(&abort_flag) != 0;

@@ -132,6 +132,34 @@ def test_many_norms(rows, width, add):
     assert torch.equal(x, s)
 
 
+@pytest.mark.parametrize("add", [None, "float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width", [(2000, 5124), (1800, 5122), (1200, 8192), (1300, 10244), (1301, 12300)])
+def test_many_long_norms(rows, width, add):
+    """Long enough for a ring of rows, in pieces of eight, four and one."""
+    test_many_norms(rows, width, add)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("width", [7, 96, 5000])
+def test_gates_at_the_ends(width, act, dtype):
+    """Gates whose square or exponential is no 32-bit number: the unit is then g u or 0.  And gates that are no number."""
+    gate_up = torch.ones(6, 2 * width, device=DEV)
+    gate_up[0, :width], gate_up[0, width:] = 2.0 ** 100, 2.0 ** -99
+    gate_up[0, 1] = 2.0 ** 99
+    gate_up[1, :width] = -2.0 ** 100
+    gate_up[1, 2], gate_up[1, width + 2] = 2.0 ** 100, 2.0 ** -100
+    gate_up[2, :width] = -200
+    gate_up[3, 3], gate_up[4, 3], gate_up[5, width + 3] = float("inf"), float("nan"), float("inf")
+    codes, scales, whole = room(6, width)
+    ops().swiglu_int8(codes, scales, gate_up.to(DT[dtype]), act)
+    assert codes[0].tolist() == [127] + [64] + [127] * (width - 2)  # 63.5 goes to the even one
+    assert abs(scales[0].item() * 127 / 2 - 1) < 2.0 ** -20
+    assert codes[1].tolist() == [0, 0, 127] + [0] * (width - 3)
+    assert not bool(codes[2].any()) and scales[2].item() == 2.0 ** -126
+    assert not bool(codes[3:].any()) and bool(torch.isnan(scales[3:]).all())
+
+
 def gate_formula(gate_up, act):
     g, u = gate_up.double().chunk(2, dim=1)
     if act == "silu":

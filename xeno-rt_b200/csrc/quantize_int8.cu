@@ -417,7 +417,19 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
 // 16-byte boundary of a stream comes by one bulk copy, the few elements outside are put beside it by the lanes of the warp that
 // asks for the copy.
 constexpr int RING_MOST = 8;
-constexpr int RING_LEAST = 6 * 1024;  // bytes of a row: shorter ones are served as well by many small blocks
+
+// Which launches take the ring: enough rows for every block to have several, and rows long enough (`stage` bytes) that few of
+// them fill a multiprocessor; shorter ones are served as well by many small blocks.  Measured on a B200 (microseconds, ring /
+// a block a row): bfloat16 rows of 1,000 (2 KB), 4,096 of them, 6.0 / 4.6; gates of 2 x 14,336, 2,048 of them, 29.5 / 47.
+// Norms read the weight again for every row (from the L2), which asks for longer ones.  Without an addition 2,048 rows of 4,096
+// (16 KB) 12.7 / 11.7, of 5,120 14.1 / 14.4, of 8,192 18.9 / 22.7, 1,200 of 5,120 9.7 / 9.4, 600 of 8,192 8.9 / 9.0; with one
+// 4,096 rows of 8,192 and bfloat16 (48 KB) 62 / 58, and float32 (64 KB) 76 / 82, 1,200 of 14,336 and bfloat16 (84 KB) 38 / 40,
+// 600 of 8,192 and float32 17.6 / 15.3.
+template <class ROWS, int VEC>
+inline bool ring_pays(int n, int grid, int stage) {
+  if (!ROWS::NORMED || VEC == 1) return n > grid && stage >= 6 * 1024;
+  return n > 4 * ROWS::STREAMS * grid && stage >= (ROWS::STREAMS == 2 ? 60 : 20) * 1024;
+}
 // Threads of a block by the values a thread holds: 32 of them need more registers than 1,024 threads have.
 constexpr int ring_threads(int per) { return per > 16 ? 832 : 1024; }
 template <class ROWS, int I>
@@ -594,7 +606,7 @@ int launch_quantize_ring(int8_t* codes, float* scales, const ROWS& rows, int n, 
   int stages = room / blocks / stage;
   if (stages > RING_MOST) stages = RING_MOST;
   const int grid = blocks * multiprocessors();
-  taken = stages >= 2 && n > (ROWS::NORMED && VEC > 1 ? 8 : 1) * grid && stage >= RING_LEAST;
+  taken = stages >= 2 && ring_pays<ROWS, VEC>(n, grid, stage);
   if (!taken) return XRT_OK;
   const cudaError_t err = allow_shared_memory_once<kernel>(room);
   if (err != cudaSuccess) return (int)err;

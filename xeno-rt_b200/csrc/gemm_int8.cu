@@ -14,8 +14,13 @@
 //               patches of 32 rows x 128 bytes to shared memory, which a TMA store takes (or a TMA reduction adds into the
 //               output), while the MMA warp fills the other accumulator.  Outputs whose rows do not begin every 16
 //               bytes are stored by the warp, a row of 32 columns at a time.
+// What bounds it: the tensor pipe, 93 percent of whose cycles are taken while a block runs (2,048 rows of 28,672 outputs, 4,096
+// inputs 145-150 us; 8,192 546, 3,527 TOP/s, until the power limit lowers the clock: 655 in a loop of seconds).  Products of one
+// wave of tiles are their walk over K and the ends: 512 rows of 4,096, 4,096 11.2 us, 333 of 5,003, 1,999 10.1 (of 5,008, 2,048,
+// whose output rows begin every 16 bytes, 7.7).  Few rows: see there.
+//
 // Every wait on an mbarrier is bounded.  A wait that runs out raises the error flag and an abort flag in shared memory; all
-// roles leave their loops, the block frees its TMEM and returns.
+// roles leave their loops, the block waits for its copies in flight (bounded too), frees its TMEM and returns.
 #include <stddef.h>
 
 #include <type_traits>
@@ -301,6 +306,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 
   fence_before();
   __syncthreads();
+  if (*abort_flag && rank == 0 && threadIdx.x == 0) mbar_wait_copies(full, STAGES, abort_flag);  // (a pair's copies: all of them)
   if (PAIR) cluster_sync();  // neither block leaves while the other may still arrive on its barriers or read its shared memory
   if (warp == 2) {
     fence_after();
@@ -400,6 +406,10 @@ int launch_gemm_int8(const Int8Product& p, cudaStream_t stream) {
 // warp 4 owns the TMEM and issues the MMAs; warps 5-8 bring the accumulators to shared memory, where all warps finish them.  A
 // kernel this short also pays for every instruction that it meets for the first time (its code comes from the L2): the
 // finish is one short loop, and while warps 5-8 wait they walk it once into a place that nobody reads.
+//
+// Measured on a B200, operands from memory, microseconds, the weight constant (bytes at 6.55 TB/s): 1 row of 6,144 outputs, 4,096
+// inputs 7.3 (3.9), 8 of 4,096, 14,336 12.3 (9.0), of 28,672, 4,096 19.6 (18.1), of 51,200, 5,120 39.4 (40.3), 64 of 28,672, 4,096
+// 21.8 (18.5), 128 of it 28.3 (20.2).  With a weight that may have just been written 0.2 to 0.9 more.
 constexpr int FEW_MAX_ROWS = 128, FEW_MAX_SPLITS = 4, FEW_MAX_STAGES = 24;
 constexpr int FEW_PRODUCERS = 4;  // (the walk below counts on four)
 constexpr int FEW_THREADS = 32 * (FEW_PRODUCERS + 1 + 4);
@@ -668,6 +678,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     }
   }
   __syncthreads();
+  if (*abort_flag && threadIdx.x == 0) mbar_wait_copies(full, stages, abort_flag);
   if (warp == FEW_PRODUCERS) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols));
@@ -681,7 +692,7 @@ static int few_shared_bytes(const FewShape& s) {
 // The tile, the parts of K and the ring of a product, from what was measured on a B200 (148 multiprocessors).
 //
 // Up to 128 weight rows a multiprocessor, one block each, the cheapest of some tiles and numbers of parts by this sum of
-// microseconds (fitted to the times of 65 products of 1 to 128 rows with every one of them: on average 2.3 percent above the
+// microseconds (fitted to the times of 65 products of 1 to 128 rows with every one of them: on average 1.9 percent above the
 // best): the longer of W from memory (6.3 TB/s in all, 0.11 TB/s into one multiprocessor, less with copies of fewer than 64
 // rows) and a block's walk over its slabs (0.15 each, or their bytes at 0.11 TB/s), half of the shorter, 0.01 a block, 0.2 for
 // each 1,000 sums that a block finishes, 0.3 where the parts of a tile meet and 0.3 for tiles of two MMAs.  The device does not
@@ -808,7 +819,10 @@ XRT_EXPORT int xrt_gemm_int8(const XrtInt8Call* call, cudaStream_t stream) {
   const xrt::Int8Product p{c.out, c.codes, c.w, c.M, c.N, c.K, c.ldx, c.ldw, c.ldo, {c.scales, c.w_scales, c.bias},
                            xrt::multiprocessors(), c.error_flag};
   if (p.sm_count <= 1) return XRT_ERR_UNSUPPORTED;
-  const bool few = c.M <= xrt::FEW_MAX_ROWS && c.N <= 65535 * 64;  // (tiles, of 64 rows at least, are a grid's second dimension)
+  // Microseconds with the few rows' kernel / tiles, operands from memory: 100 rows of 6,144 outputs, 4,096 inputs 11.1 / 11.1, of
+  // 4,096, 14,336 18.6 / 24.4, of 28,672, 4,096 26.6 / 26.0; 136 rows (with room for them) 13.2 / 11.3 and 20.3 / 24.6; 200 rows of
+  // 4,096, 14,336 54 / 24.7.  (Its tiles, of 64 weight rows at least, are a grid's second dimension.)
+  const bool few = c.M <= xrt::FEW_MAX_ROWS && c.N <= 65535 * 64;
   if (c.mode == 1)
     return few ? xrt::launch_gemm_int8_few<1, float>(p, c.constant_weight, stream) : xrt::launch_gemm_int8<1, float>(p, stream);
   XRT_DISPATCH_DTYPE(c.out_dtype, TO, {

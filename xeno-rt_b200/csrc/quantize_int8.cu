@@ -13,6 +13,13 @@
 // Few rows (steps): a block a row, its loads all in flight together.  More rows than blocks: blocks take every so many-th
 // row from a ring in shared memory that bulk copies fill ahead (quantize_int8_ring_kernel), so that the memory is asked for the
 // next rows while a block meets.  Rows beyond what 1,024 threads hold are walked twice.
+//
+// What bounds it: many long rows the memory, and beside it the instructions that a multiprocessor issues (hence Two, largest_of
+// and sigmoid below: gates 64 -> 51 us, 4,096 plain rows of 8,192 22.6 -> 20.6); few rows the time of one load, one meeting and
+// one store.  Measured on a B200, operands from memory, microseconds (bytes that it cannot do without at 6.55 TB/s): norm after
+// an addition of 1 row of 4,096 2.2, of 2,048 16.3 (14.1), of 8,191 of 5,120, float32 79-86 (83); gate of 8 rows of 14,336
+// units 2.8, of 2,048 29.6 (22.4), of 2,000 of 25,600 51 (39); plain rows, 64 of 4,096 1.5, 4,096 of 8,192 20.7 (15.4).
+// Rows of a width or an address that allows single values only take longer: norm of 2,047 of 4,095 37 (16.6).
 #include <stddef.h>
 
 #include <type_traits>
@@ -576,7 +583,10 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
     }
     finish_row<ROWS, VEC, ITEMS>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
     if (++s == stages) { s = 0; turn ^= 1; }
-    if (given_up) break;
+    if (given_up) {
+      if (threadIdx.x == 0) mbar_wait_copies(full, stages, &abort_flag);
+      break;
+    }
   }
 }
 
@@ -618,6 +628,8 @@ template <class ROWS, int VEC>
 int launch_quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag, cudaStream_t stream) {
   bool taken = false;
   int status = XRT_OK;
+  // Microseconds with 16 / 32 values a thread: 2,048 gates of 14,336 units 29.8 / 34.8, 600 13.2 / 14.1; plain rows between
+  // 20.5 / 19.2 (8,191 of 4,096) and 8.2 / 8.0 (600 of 14,336).
   if (width <= 16 * 1024)
     status = launch_quantize_ring<ROWS, VEC, 16>(codes, scales, rows, n, width, ld_codes, error_flag, stream, taken);
   else if (width <= 32 * 1024)
@@ -628,6 +640,8 @@ int launch_quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int w
     launch_kernel(kernel, dim3(n), dim3(threads), 0, stream, codes, scales, rows, width, ld_codes);
     return launch_status();
   };
+  // The fewest values a thread that 1,024 threads allow, which keeps the most loads in flight.  Microseconds with 8 / 16 a thread:
+  // norm of 1 row of 4,096 2.0 / 2.25, of 2,048 16.4 / 18.5, gate of 600 of 8,192 8.1 / 9.2, 600 plain rows of 8,192 5.3 / 5.5.
   if (width <= 8 * 1024) return launch(quantize_int8_kernel<ROWS, VEC, 8 / VEC>, 8);
   if (width <= 16 * 1024) return launch(quantize_int8_kernel<ROWS, VEC, 16 / VEC>, 16);
   if (width <= 32 * 1024) return launch(quantize_int8_kernel<ROWS, VEC, 32 / VEC>, 32);

@@ -53,6 +53,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
   return false;
 }
+// What a block does whose `abort_flag` is raised, before it leaves: waits until the copies that it has asked for have landed in its
+// shared memory, on the barriers that hear of them, whatever phase each is in (a phase with nothing to come runs out after
+// 1,024 polls).  For one thread.
+__device__ __forceinline__ void mbar_wait_copies(uint64_t* full, int count, volatile int* abort_flag) {
+  for (int s = 0; s < 2 * count; ++s) mbar_wait(smem_u32(&full[s >> 1]), s & 1, abort_flag);
+}
 // A tile of a two-dimensional tensor map into shared memory; c0 is the innermost coordinate (its
 // byte offset must be a multiple of 16).  No multicast: the tile goes to this block only.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {

@@ -118,3 +118,29 @@ def test_a_random_model_is_the_one_of_its_folder(tmp_path):
     logits = [_whole(Engine(m, max_tokens=256), prompt) for m in (Model.load(folder, weights="int8"),
                                                                   Model.random(raw, seed=seed, weights="int8"))]
     assert np.array_equal(*logits)
+
+
+def test_layers_that_share_their_tensors(setups):
+    """Two layers built from the same tensors, and from copies of them."""
+    from xeno_rt_b200.config import load_config
+    from xeno_rt_b200.core import parse_dtype
+    from xeno_rt_b200.engine import Engine, Model
+    from xeno_rt_b200.weights import load_weights
+    folder, prompts, _ = setups["tiny-wide"]
+    arch, config = load_config(folder)
+    logits = []
+    for share in (True, False):
+        spec = arch.build_spec(config)
+        tensors = load_weights(folder, spec.expected_tensors(), parse_dtype("bfloat16"), "cuda:0", spec.ignorable_tensors,
+                               fused_groups=spec.fused_groups())
+        if share:
+            spec.layers[1] = spec.layers[0]
+        else:
+            for name, (_, part) in spec.layers[0].parts.items():
+                for role, source in part.weights.items():
+                    tensors[spec.layers[1].parts[name][1].weights[role]].copy_(tensors[source])
+        model = Model(spec, tensors, parse_dtype("bfloat16"), "cuda:0", config, weights="int8")
+        assert not any(n in tensors for _, part in spec.layers[0].parts.values() if part.kind in ("attention", "swiglu")
+                       for n in part.weights.values())
+        logits.append(_whole(Engine(model, max_tokens=64 * 24), prompts[0]))
+    assert np.array_equal(*logits)

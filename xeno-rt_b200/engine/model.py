@@ -51,6 +51,11 @@ class Model:
         self.max_positions = spec.max_positions
 
         shared = getattr(tensors, "fused", {})
+        readers = {}  # how many parts still have to be built from a tensor
+        for part_spec in [spec.embedding, spec.final_norm, spec.lm_head, *spec.stream_parts.values(),
+                          *(part for layer in spec.layers for _, part in layer.parts.values())]:
+            for name in part_spec.weights.values():
+                readers[name] = readers.get(name, 0) + 1
 
         def build(role, part_spec):
             cls = part_class(role, part_spec.kind)
@@ -63,9 +68,11 @@ class Model:
             part = cls(part_spec.params, weights, dtype, self.device)
             if self.weights_format == "int8" and hasattr(part, "use_int8"):
                 part.use_int8()
-                for name in part_spec.weights.values():  # the stored form of its matrices is needed no more
-                    tensors.pop(name)
-                for names in [n for n in shared if set(n) <= set(part_spec.weights.values())]:
+                for name in part_spec.weights.values():
+                    readers[name] -= 1
+                    if readers[name] == 0:  # the stored form of the matrix is needed no more
+                        tensors.pop(name)
+                for names in [n for n in shared if set(n) <= set(part_spec.weights.values()) and not any(readers[r] for r in n)]:
                     shared.pop(names)
             return part
 
@@ -74,6 +81,8 @@ class Model:
         self.layers = [LayerParts({name: build(role, part) for name, (role, part) in l.parts.items()},
                                   {name: role for name, (role, _) in l.parts.items()}) for l in spec.layers]
         self.arrangements = [part_class("arrangement", l.arrangement) for l in spec.layers]
+        if weights == "int8":
+            torch.cuda.synchronize(self.device)  # products may read their weights before the kernels before them are done
         self.final_norm = build("norm", spec.final_norm)
         self.lm_head = build("lm_head", spec.lm_head)
         self.error_flag = ops.device_state(self.device)[0]

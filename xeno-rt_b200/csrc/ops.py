@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import dataclasses
+import functools
 import struct
 import threading
 
@@ -333,8 +334,13 @@ class Gate:
         return ctypes.byref(_GateOptions(_ptr(self.bias, "bias", torch.float32), float(self.limit), float(self.alpha)))
 
 
+@functools.lru_cache(maxsize=16)
+def _named_gate(act: str) -> Gate:
+    return Gate(act)
+
+
 def _gate_of(act) -> Gate:
-    return act if isinstance(act, Gate) else Gate(act)
+    return _named_gate(act) if isinstance(act, str) else act if isinstance(act, Gate) else Gate(act)
 
 
 def _gate_code(gate: Gate, mode: str) -> int:
@@ -1777,9 +1783,10 @@ def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
     what = "swiglu_int8"
     gate = _gate_of(act)
     code = _gate_code(gate, "swiglu")
-    if gate_up.dim() != 2 or gate_up.shape[1] % 2:
+    shape = gate_up.shape
+    if len(shape) != 2 or shape[1] % 2:
         raise KernelError(f"{what}: gate_up must be [rows, 2 * width]")
-    n, width = gate_up.shape[0], gate_up.shape[1] // 2
+    n, width = shape[0], shape[1] // 2
     ld = _codes(codes, "codes", what, n, width)
     options = gate.options(width)  # (a reference, which the call needs alive)
     call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), 0, 0, 0,
@@ -1795,14 +1802,16 @@ def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None, const
     float32 [n, width], ``weight`` float32 or bfloat16 [width].  ``constant_weight``: the weight is a model's, which no kernel
     that may still run has written: it is then read while the kernel before finishes."""
     what = "rmsnorm_int8"
-    if x.dim() != 2 or tuple(weight.shape) != (x.shape[1],):
+    shape = x.shape
+    if len(shape) != 2 or weight.shape != shape[1:]:
         raise KernelError(f"{what}: x must be [rows, width] and weight [width]")
-    if add is None and out is not None:
-        raise KernelError(f"{what}: out is the sum of x and add, and there is no add")
-    n, width = x.shape
-    if add is not None:
+    n, width = shape
+    if add is None:
+        if out is not None:
+            raise KernelError(f"{what}: out is the sum of x and add, and there is no add")
+    else:
         out = x if out is None else out
-        if add.shape != x.shape or out.shape != x.shape:
+        if add.shape != shape or out.shape != shape:
             raise KernelError(f"{what}: add and out must have the shape of x")
     ld = _codes(codes, "codes", what, n, width)
     call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),

@@ -16,8 +16,8 @@
 //               bytes are stored by the warp, a row of 32 columns at a time.
 // What bounds it: the tensor pipe, 93 percent of whose cycles are taken while a block runs (2,048 rows of 28,672 outputs, 4,096
 // inputs 145-150 us; 8,192 546, 3,527 TOP/s, until the power limit lowers the clock: 655 in a loop of seconds).  Products of one
-// wave of tiles are their walk over K and the ends: 512 rows of 4,096, 4,096 11.2 us, 333 of 5,003, 1,999 10.1 (of 5,008, 2,048,
-// whose output rows begin every 16 bytes, 7.7).  Few rows: see there.
+// wave of tiles are their walk over K and the ends: 512 rows of 4,096, 4,096 11.2 us, 333 of 5,003, 1,999 7.7 (of 5,008, 2,048,
+// whose output rows begin every 16 bytes, 7.2).  Few rows: see there.
 //
 // Every wait on an mbarrier is bounded.  A wait that runs out raises the error flag and an abort flag in shared memory; all
 // roles leave their loops, the block waits for its copies in flight (bounded too), frees its TMEM and returns.
@@ -90,7 +90,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   using Shape = Int8Shape<PAIR, BN>;
   constexpr int STAGES = Shape::STAGES, TILE_ROWS = (PAIR ? 2 : 1) * I8_BM;
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   unsigned char* a_stages = smem;
   unsigned char* b_stages = smem + STAGES * Shape::A_BYTES;
   unsigned char* staging = smem + STAGES * Shape::STAGE_BYTES;
@@ -362,14 +362,15 @@ int launch_gemm_int8_tiled(const Int8Product& p, cudaStream_t stream) {
 }
 
 // The tile: 0 pairs of 256 x 256, 1 pairs of 256 x 128, 2 single blocks of 128 x 256, 3 of 128 x 128: the least of what it takes
-// to begin and end, and the longer of the rounds of tiles (microseconds a 128-wide slab of K) and the operands from memory,
-// as measured on a B200 with the operands in memory.  Microseconds (0 / 1 / 2 / 3): 256 rows of 6,144 outputs, 4,096 inputs
-// 15.5 / 11.5 / 17.1 / 11.8; 333 of 6,144, 4,096 16.4 / 16.3 / 17.0 / 12.0; 512 of 4,096, 14,336 39.1 / 25.5 / 44.6 / 28.9;
-// 8,192 of 28,672, 4,096 546 / 686 / 608 / 851 (3,527 TOP/s).
+// to begin and end, the longer of the rounds of tiles (microseconds a 128-wide slab of K) and the operands from memory, and a fifth of
+// the shorter; fitted to the times of 104 products of 136 to 8,192 rows with all four on a B200, the operands in memory (the
+// choice is on average 0.1 percent above the best of them).  Microseconds (0 / 1 / 2 / 3): 256 rows of 6,144 outputs, 4,096 inputs
+// 15.1 / 11.6 / 16.6 / 11.4; 256 of 28,672, 4,096 31.6 / 33.8 / 34.9 / 36.9; 512 of 4,096, 14,336 39.0 / 26.0 / 44.6 / 28.7; 333 of
+// 10,240, 5,120 29.7 / 26.9 / 21.3 / 22.5; 8,192 of 28,672, 4,096 565 / 703 / 626 / 839 (546 at best, 3,527 TOP/s).
 static int int8_form(const Int8Product& p) {
   constexpr int rows[4] = {256, 256, 128, 128}, columns[4] = {256, 128, 256, 128};
-  constexpr double slab_us[4] = {0.281, 0.168, 0.35, 0.21}, ends_us[4] = {6.5, 6.1, 5.9, 5.1};
-  const double memory_us = ((double)p.M + p.N) * p.K / 5e6;
+  constexpr double slab_us[4] = {0.26, 0.154, 0.302, 0.204}, ends_us[4] = {6.6, 8.1, 8.2, 4.0};
+  const double memory_us = ((double)p.M + p.N) * p.K / 6.3e6;
   const long long slabs = (p.K + I8_BK - 1) / I8_BK;
   int best = 0;
   double least = 0;
@@ -377,7 +378,8 @@ static int int8_form(const Int8Product& p) {
     const long long tiles = (long long)((p.M + rows[form] - 1) / rows[form]) * ((p.N + columns[form] - 1) / columns[form]);
     const int units = rows[form] == 256 ? p.sm_count / 2 : p.sm_count;
     const double walk_us = (double)((tiles + units - 1) / units * slabs) * slab_us[form];
-    const double cost = ends_us[form] + (walk_us > memory_us ? walk_us : memory_us);
+    const double longer = walk_us > memory_us ? walk_us : memory_us;
+    const double cost = ends_us[form] + longer + 0.2 * (walk_us + memory_us - longer);
     if (form == 0 || cost < least) { least = cost; best = form; }
   }
   return best;
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
 gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, TO* out,
                      const FewShape shape, const Int8Scales scales, int* error_flag) {
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   const int stages = shape.stages, nb = shape.nb, splits = shape.splits, slabs = shape.slabs;
   const int w_bytes = few_w_bytes(shape), x_bytes = nb * I8_BK, stage_bytes = few_stage_bytes(shape);
   unsigned char* tail = smem + few_ring_bytes(shape);
@@ -692,7 +694,7 @@ static int few_shared_bytes(const FewShape& s) {
 // The tile, the parts of K and the ring of a product, from what was measured on a B200 (148 multiprocessors).
 //
 // Up to 128 weight rows a multiprocessor, one block each, the cheapest of some tiles and numbers of parts by this sum of
-// microseconds (fitted to the times of 65 products of 1 to 128 rows with every one of them: on average 1.9 percent above the
+// microseconds (fitted to the times of 65 products of 1 to 128 rows with every one of them: on average 1.7 percent above the
 // best): the longer of W from memory (6.3 TB/s in all, 0.11 TB/s into one multiprocessor, less with copies of fewer than 64
 // rows) and a block's walk over its slabs (0.15 each, or their bytes at 0.11 TB/s), half of the shorter, 0.01 a block, 0.2 for
 // each 1,000 sums that a block finishes, 0.3 where the parts of a tile meet and 0.3 for tiles of two MMAs.  The device does not

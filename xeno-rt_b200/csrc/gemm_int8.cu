@@ -367,27 +367,29 @@ int launch_gemm_int8_tiled(const Int8Product& p, cudaStream_t stream) {
 // choice is on average 0.1 percent above the best of them).  Microseconds (0 / 1 / 2 / 3): 256 rows of 6,144 outputs, 4,096 inputs
 // 15.1 / 11.6 / 16.6 / 11.4; 256 of 28,672, 4,096 31.6 / 33.8 / 34.9 / 36.9; 512 of 4,096, 14,336 39.0 / 26.0 / 44.6 / 28.7; 333 of
 // 10,240, 5,120 29.7 / 26.9 / 21.3 / 22.5; 8,192 of 28,672, 4,096 565 / 703 / 626 / 839 (546 at best, 3,527 TOP/s).
-static int int8_form(const Int8Product& p) {
+struct Int8Form {
+  int form;
+  double us;
+};
+static Int8Form int8_form(const Int8Product& p) {
   constexpr int rows[4] = {256, 256, 128, 128}, columns[4] = {256, 128, 256, 128};
   constexpr double slab_us[4] = {0.26, 0.154, 0.302, 0.204}, ends_us[4] = {6.6, 8.1, 8.2, 4.0};
   const double memory_us = ((double)p.M + p.N) * p.K / 6.3e6;
   const long long slabs = (p.K + I8_BK - 1) / I8_BK;
-  int best = 0;
-  double least = 0;
+  Int8Form best = {0, 0};
   for (int form = 0; form < 4; ++form) {
     const long long tiles = (long long)((p.M + rows[form] - 1) / rows[form]) * ((p.N + columns[form] - 1) / columns[form]);
     const int units = rows[form] == 256 ? p.sm_count / 2 : p.sm_count;
     const double walk_us = (double)((tiles + units - 1) / units * slabs) * slab_us[form];
     const double longer = walk_us > memory_us ? walk_us : memory_us;
-    const double cost = ends_us[form] + longer + 0.2 * (walk_us + memory_us - longer);
-    if (form == 0 || cost < least) { least = cost; best = form; }
+    const double us = ends_us[form] + longer + 0.2 * (walk_us + memory_us - longer);
+    if (form == 0 || us < best.us) best = {form, us};
   }
   return best;
 }
 
 template <int MODE, typename TO>
-int launch_gemm_int8(const Int8Product& p, cudaStream_t stream) {
-  const int form = int8_form(p);
+int launch_gemm_int8(const Int8Product& p, int form, cudaStream_t stream) {
   if (form == 0) return launch_gemm_int8_tiled<MODE, true, 256, TO>(p, stream);
   if (form == 1) return launch_gemm_int8_tiled<MODE, true, 128, TO>(p, stream);
   if (form == 2) return launch_gemm_int8_tiled<MODE, false, 256, TO>(p, stream);
@@ -655,7 +657,8 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         sums[0] += lo.x; sums[1] += lo.y; sums[2] += lo.z; sums[3] += lo.w;
         sums[4] += hi.x; sums[5] += hi.y; sums[6] += hi.z; sums[7] += hi.w;
       }
-      const float4 s_lo = *reinterpret_cast<const float4*>(row_scales + eight * 8), s_hi = *reinterpret_cast<const float4*>(row_scales + eight * 8 + 4);
+      const float4 s_lo = *reinterpret_cast<const float4*>(row_scales + eight * 8);
+      const float4 s_hi = *reinterpret_cast<const float4*>(row_scales + eight * 8 + 4);
       const float by_column = column_scales[row_lo + local], bias = biases[row_lo + local];
       const float factors[8] = {s_lo.x, s_lo.y, s_lo.z, s_lo.w, s_hi.x, s_hi.y, s_hi.z, s_hi.w};
       // rows beyond M, and all rows of the first walk, go nowhere; what is added into is asked for before the first store,
@@ -758,22 +761,44 @@ static void plan_few(FewShape& s, int K, int sm_count) {
   }
 }
 
-template <int MODE, typename TO>
-int launch_gemm_int8_few(const Int8Product& p, int constant_weight, cudaStream_t stream) {
-  constexpr auto kernel = gemm_int8_few_kernel<MODE, TO>;
-  const cudaError_t err = allow_shared_memory_once<kernel>(FEW_SHARED_ONE);
-  if (err != cudaSuccess) return (int)err;
+static FewShape few_shape(const Int8Product& p) {
   FewShape shape = {};
   shape.M = p.M; shape.N = p.N; shape.ldo = p.ldo;
   shape.nb = (p.M + 15) / 16 * 16;
-  shape.early = constant_weight;
   plan_few(shape, p.K, p.sm_count);
+  shape.k_each = shape.k_iters / shape.splits;
+  shape.k_more = shape.k_iters - shape.k_each * shape.splits;
+  return shape;
+}
+
+// Microseconds of a product by this kernel, for the choice between it and tiles: to begin and end, the longer of W from memory and
+// of what a multiprocessor's blocks copy (the codes again for every tile), some of the shorter, and the sums that a block
+// finishes; fitted, together with int8_form's, to the times of 188 products of 1 to 128 rows by both, in bfloat16.  The choice is
+// on average 0.2 percent above the better one, and 8 at most; this kernel for all of them 5, and 50 at most.  Microseconds, this
+// kernel / tiles: 48 rows of 10,240 outputs, 5,120 inputs 13.1 / 14.4, 96 16.4 / 14.6; 128 of 4,096, 14,336 18.4 / 24.5, of
+// 6,400, 512 6.4 / 4.3, of 51,200, 5,120 72 / 47; 64 of 102,400, 1,024 29 / 24.  Up to 16 rows, and up to 48 where every block has a multiprocessor of its
+// own, it was never behind, and is not compared.
+static double few_us(const FewShape& s, int K, int sm_count) {
+  const int blocks = (s.N + s.rows - 1) / s.rows * s.splits, each = (blocks + sm_count - 1) / sm_count;
+  const int slabs = ((K + I8_BK - 1) / I8_BK + s.splits - 1) / s.splits;
+  const double into = blocks * 0.11e6, slab_us = (s.rows + s.M) * 128 / 93e3;
+  const double memory_us = (double)s.N * K / (into < 6.3e6 ? into : 6.3e6);
+  const double walk_us = each * slabs * (slab_us > 0.15 ? slab_us : 0.15);
+  const double longer = memory_us > walk_us ? memory_us : walk_us, shorter = memory_us + walk_us - longer;
+  if (each > 1) return 0.4 + longer + 0.13 * shorter + 0.2e-3 * s.rows * s.M * each;  // (blocks begin and end beside others)
+  return 3.8 + longer + 0.14 * shorter + 0.16e-3 * s.rows * s.M;
+}
+
+template <int MODE, typename TO>
+int launch_gemm_int8_few(const Int8Product& p, FewShape shape, int constant_weight, cudaStream_t stream) {
+  constexpr auto kernel = gemm_int8_few_kernel<MODE, TO>;
+  const cudaError_t err = allow_shared_memory_once<kernel>(FEW_SHARED_ONE);
+  if (err != cudaSuccess) return (int)err;
+  shape.early = constant_weight;
   CUtensorMap map_w, map_x;
   if (!make_map_int8_2d(&map_x, p.codes, p.M, p.K, p.ldx, shape.nb) || !make_map_int8_2d(&map_w, p.w, p.N, p.K, p.ldw, shape.rows))
     return XRT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t config = {};
-  shape.k_each = shape.k_iters / shape.splits;
-  shape.k_more = shape.k_iters - shape.k_each * shape.splits;
   config.gridDim = dim3((unsigned)shape.splits, (unsigned)((shape.N + shape.rows - 1) / shape.rows));
   config.blockDim = dim3(FEW_THREADS);
   config.dynamicSmemBytes = few_shared_bytes(shape);
@@ -821,13 +846,19 @@ XRT_EXPORT int xrt_gemm_int8(const XrtInt8Call* call, cudaStream_t stream) {
   const xrt::Int8Product p{c.out, c.codes, c.w, c.M, c.N, c.K, c.ldx, c.ldw, c.ldo, {c.scales, c.w_scales, c.bias},
                            xrt::multiprocessors(), c.error_flag};
   if (p.sm_count <= 1) return XRT_ERR_UNSUPPORTED;
-  // Microseconds with the few rows' kernel / tiles, operands from memory: 100 rows of 6,144 outputs, 4,096 inputs 11.1 / 11.1, of
-  // 4,096, 14,336 18.6 / 24.4, of 28,672, 4,096 26.6 / 26.0; 136 rows (with room for them) 13.2 / 11.3 and 20.3 / 24.6; 200 rows of
-  // 4,096, 14,336 54 / 24.7.  (Its tiles, of 64 weight rows at least, are a grid's second dimension.)
-  const bool few = c.M <= xrt::FEW_MAX_ROWS && c.N <= 65535 * 64;
+  // (The few rows' kernel: its tiles, of 64 weight rows at least, are a grid's second dimension.)
+  xrt::FewShape shape = {};
+  xrt::Int8Form tiles = {0, 0};
+  bool few = c.M <= xrt::FEW_MAX_ROWS && c.N <= 65535 * 64;
+  if (few) shape = xrt::few_shape(p);
+  const bool either = few && c.M > ((c.N + shape.rows - 1) / shape.rows * shape.splits > p.sm_count ? 16 : 48);
+  if (!few || either) tiles = xrt::int8_form(p);
+  if (either) few = xrt::few_us(shape, c.K, p.sm_count) <= tiles.us;
   if (c.mode == 1)
-    return few ? xrt::launch_gemm_int8_few<1, float>(p, c.constant_weight, stream) : xrt::launch_gemm_int8<1, float>(p, stream);
+    return few ? xrt::launch_gemm_int8_few<1, float>(p, shape, c.constant_weight, stream)
+               : xrt::launch_gemm_int8<1, float>(p, tiles.form, stream);
   XRT_DISPATCH_DTYPE(c.out_dtype, TO, {
-    return few ? xrt::launch_gemm_int8_few<0, TO>(p, c.constant_weight, stream) : xrt::launch_gemm_int8<0, TO>(p, stream);
+    return few ? xrt::launch_gemm_int8_few<0, TO>(p, shape, c.constant_weight, stream)
+               : xrt::launch_gemm_int8<0, TO>(p, tiles.form, stream);
   });
 }

@@ -776,8 +776,8 @@ static FewShape few_shape(const Int8Product& p) {
 // finishes; fitted, together with int8_form's, to the times of 188 products of 1 to 128 rows by both, in bfloat16.  The choice is
 // on average 0.2 percent above the better one, and 8 at most; this kernel for all of them 5, and 50 at most.  Microseconds, this
 // kernel / tiles: 48 rows of 10,240 outputs, 5,120 inputs 13.1 / 14.4, 96 16.4 / 14.6; 128 of 4,096, 14,336 18.4 / 24.5, of
-// 6,400, 512 6.4 / 4.3, of 51,200, 5,120 72 / 47; 64 of 102,400, 1,024 29 / 24.  Up to 16 rows, and up to 48 where every block has a multiprocessor of its
-// own, it was never behind, and is not compared.
+// 6,400, 512 6.4 / 4.3, of 51,200, 5,120 72 / 47; 64 of 102,400, 1,024 29 / 24.  Up to 16 rows, and up to 48 where every block
+// has a multiprocessor of its own, it was never behind, and is not compared.
 static double few_us(const FewShape& s, int K, int sm_count) {
   const int blocks = (s.N + s.rows - 1) / s.rows * s.splits, each = (blocks + sm_count - 1) / sm_count;
   const int slabs = ((K + I8_BK - 1) / I8_BK + s.splits - 1) / s.splits;

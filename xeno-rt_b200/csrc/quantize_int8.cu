@@ -427,15 +427,14 @@ constexpr int RING_MOST = 8;
 
 // Which launches take the ring: enough rows for every block to have several, and rows long enough (`stage` bytes) that few of
 // them fill a multiprocessor; shorter ones are served as well by many small blocks.  Measured on a B200 (microseconds, ring /
-// a block a row): bfloat16 rows of 1,000 (2 KB), 4,096 of them, 6.0 / 4.6; gates of 2 x 14,336, 2,048 of them, 29.5 / 47.
-// Norms read the weight again for every row (from the L2), which asks for longer ones.  Without an addition 2,048 rows of 4,096
-// (16 KB) 12.7 / 11.7, of 5,120 14.1 / 14.4, of 8,192 18.9 / 22.7, 1,200 of 5,120 9.7 / 9.4, 600 of 8,192 8.9 / 9.0; with one
-// 4,096 rows of 8,192 and bfloat16 (48 KB) 62 / 58, and float32 (64 KB) 76 / 82, 1,200 of 14,336 and bfloat16 (84 KB) 38 / 40,
-// 600 of 8,192 and float32 17.6 / 15.3.
+// a block a row): bfloat16 rows of 1,000 (2 KB), 4,096 of them, 6.0 / 4.6; gates of 2 x 14,336, 2,048 of them, 29.5 / 47; norms
+// without an addition, 600 of 4,096 (16 KB) 4.9 / 5.3, 2,048 10.6 / 11.7, 2,048 of 8,192 16.8 / 22.7, 8,191 of 14,336 90 / 136.
+// With an addition the sum is written as well, and longer rows are asked for: 4,096 of 8,192 and bfloat16 (48 KB) 67 / 58, and
+// float32 (64 KB) 74 / 82, 600 14.9 / 15.3, 1,200 of 14,336 and bfloat16 (84 KB) 34 / 40.
 template <class ROWS, int VEC>
 inline bool ring_pays(int n, int grid, int stage) {
-  if (!ROWS::NORMED || VEC == 1) return n > grid && stage >= 6 * 1024;
-  return n > 4 * ROWS::STREAMS * grid && stage >= (ROWS::STREAMS == 2 ? 60 : 20) * 1024;
+  if (ROWS::STREAMS == 1 || VEC == 1) return n > grid && stage >= 6 * 1024;
+  return n > 3 * grid && stage >= 60 * 1024;
 }
 // Threads of a block by the values a thread holds: 32 of them need more registers than 1,024 threads have.
 constexpr int ring_threads(int per) { return per > 16 ? 832 : 1024; }
@@ -517,6 +516,16 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
   const int stride = (int)blockDim.x * VEC, stage_bytes = ring_stage<ROWS>(width), room0 = ring_room<ROWS, 0>(width);
   const int lane = threadIdx.x & 31;
   __syncthreads();
+  // A thread has the same columns of every row: it keeps their weights, where they leave room for the values.
+  constexpr bool KEEPS = ROWS::NORMED && VEC * ITEMS <= 16;
+  float kept[KEEPS ? ITEMS : 1][VEC];
+  auto keep = [&]() {
+    if constexpr (KEEPS) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) rows.template ahead<VEC>((int)threadIdx.x * VEC + i * stride, width, kept[i]);
+    }
+  };
+  if (rows.early) keep();
   rows.wait();
   auto fetch = [&](int row, int s) {  // the first warp
     unsigned char* place = ring + s * stage_bytes;
@@ -540,6 +549,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
   };
   if (threadIdx.x < 32)
     for (int s = 0, row = blockIdx.x; s < stages && row < n; ++s, row += gridDim.x) fetch(row, s);
+  if (!rows.early) keep();
   int s = 0, turn = 0, side = 0;
   for (int row = blockIdx.x; row < n; row += gridDim.x) {
     if (!mbar_wait(smem_u32(&full[s]), turn, &abort_flag)) {
@@ -564,7 +574,9 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
     for (int i = 0; i < ITEMS; ++i) {
       const int c = (int)threadIdx.x * VEC + i * stride;
       if (!ROWS::NORMED || c < width) {
-        if constexpr (ROWS::NORMED) {
+        if constexpr (KEEPS) {
+          rows.template settle<VEC, false>(row, c, width, kept[i], v[i], squares);
+        } else if constexpr (ROWS::NORMED) {
           float w[VEC];
           rows.template ahead<VEC>(c, width, w);
           rows.template settle<VEC, false>(row, c, width, w, v[i], squares);

@@ -361,7 +361,7 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
   __shared__ uint32_t most[32];
   __shared__ float sums[32];
   constexpr int KEPT = ITEMS > 0 ? ITEMS : 1;
-  constexpr bool AHEAD = ITEMS > 0 && ITEMS * VEC <= 8;
+  constexpr bool AHEAD = ITEMS > 0 && ITEMS * VEC <= 16;
   pdl_trigger();
   float w[KEPT][VEC], v[KEPT][VEC];
   const int stride = (int)blockDim.x * VEC;

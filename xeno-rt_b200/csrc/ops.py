@@ -1735,14 +1735,20 @@ def _run_int8(what: str, tensors, launcher, call) -> None:
     _check(status, what)
 
 
+_error_flags_at: dict = {}  # their addresses
+
+
 def _error_flag_pointer(index: int) -> int:
     """A device's error flag for a launch; 0 (the kernel reports nothing) where it would have to be made inside a capture."""
-    flag = _error_flags.get(index)
-    if flag is None:
-        if index < 0 or torch.cuda.is_current_stream_capturing():
-            return 0
-        flag = error_flag(torch.device("cuda", index))
-    return flag.data_ptr()
+    at = _error_flags_at.get(index)
+    if at is None:
+        flag = _error_flags.get(index)
+        if flag is None:
+            if index < 0 or torch.cuda.is_current_stream_capturing():
+                return 0
+            flag = error_flag(torch.device("cuda", index))
+        at = _error_flags_at[index] = flag.data_ptr()
+    return at
 
 
 def _codes(t, name: str, what: str, rows: int, width: int) -> int:
@@ -1753,6 +1759,15 @@ def _codes(t, name: str, what: str, rows: int, width: int) -> int:
     if (width > 1 and step != 1) or (rows > 1 and not width <= distance < 1 << 31):
         raise KernelError(f"{what}: the rows of {name} must be contiguous and less than 2^31 bytes apart")
     return distance if rows > 1 else -(-width // 16) * 16
+
+
+def _whole(t, name: str, dtype=None) -> int:
+    """The address of a tensor without gaps (``_run_int8`` looks at its device)."""
+    if not t.is_contiguous():
+        raise KernelError(f"{name} is not contiguous")
+    if dtype is not None and t.dtype is not dtype:
+        raise KernelError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    return t.data_ptr()
 
 
 def _vector(t, name: str, what: str, size: int) -> int:
@@ -1771,7 +1786,7 @@ def quantize_rows(codes, scales, x) -> None:
         raise KernelError(f"{what}: x must be [rows, width]")
     n, width = x.shape
     ld = _codes(codes, "codes", what, n, width)
-    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x"), 0, 0, 0, 0,
+    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _whole(x, "x"), 0, 0, 0, 0,
                            _error_flag_pointer(x.get_device()), n, width, ld, _code(x.dtype), 0, 0, 0, 0, 0.0)
     _run_int8(what, (x, codes, scales), _kernels().xrt_quantize_rows, call)
 
@@ -1789,7 +1804,7 @@ def swiglu_int8(codes, scales, gate_up, act="silu") -> None:
     n, width = shape[0], shape[1] // 2
     ld = _codes(codes, "codes", what, n, width)
     options = gate.options(width)  # (a reference, which the call needs alive)
-    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(gate_up, "gate_up"), 0, 0, 0,
+    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _whole(gate_up, "gate_up"), 0, 0, 0,
                            0 if options is None else ctypes.addressof(options._obj), _error_flag_pointer(gate_up.get_device()),
                            n, width, ld, _code(gate_up.dtype), 0, 0, code, 0, 0.0)
     _run_int8(what, (gate_up, codes, scales, gate.bias), _kernels().xrt_swiglu_int8, call)
@@ -1814,10 +1829,10 @@ def rmsnorm_int8(codes, scales, x, weight, eps: float, add=None, out=None, const
         if add.shape != shape or out.shape != shape:
             raise KernelError(f"{what}: add and out must have the shape of x")
     ld = _codes(codes, "codes", what, n, width)
-    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _ptr(x, "x", torch.float32), _ptr(add, "add"),
-                           _ptr(out, "out", torch.float32), _ptr(weight, "weight"), 0, _error_flag_pointer(x.get_device()),
-                           n, width, ld, 0, 0 if add is None else _code(add.dtype), _code(weight.dtype), 0,
-                           1 if constant_weight else 0, eps)
+    call = _pack_int8_rows(codes.data_ptr(), _vector(scales, "scales", what, n), _whole(x, "x", torch.float32),
+                           0 if add is None else _whole(add, "add"), 0 if add is None else _whole(out, "out", torch.float32),
+                           _whole(weight, "weight"), 0, _error_flag_pointer(x.get_device()), n, width, ld, 0,
+                           0 if add is None else _code(add.dtype), _code(weight.dtype), 0, 1 if constant_weight else 0, eps)
     _run_int8(what, (x, codes, scales, weight, add, out), _kernels().xrt_rmsnorm_int8, call)
 
 

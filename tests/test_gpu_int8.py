@@ -132,6 +132,27 @@ def test_many_norms(rows, width, add):
     assert torch.equal(x, s)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width", [(500, 4099), (700, 4102), (301, 7001), (160, 20003)])
+def test_many_rows_into_codes_that_lie_anywhere(rows, width, dtype):
+    """Codes without gaps between rows, from any byte on: what lies before and behind them stays."""
+    for shift in (0, 1, 2):
+        buffer = torch.full((rows * width + 8,), 99, dtype=torch.int8, device=DEV)
+        codes, scales = buffer[shift:shift + rows * width].view(rows, width), torch.empty(rows, device=DEV)
+        beside, beside_scales, whole = room(rows, width)
+        x = normal(rows, width, seed=75, dtype=DT[dtype])
+        ops().quantize_rows(codes, scales, x)
+        ops().quantize_rows(beside, beside_scales, x)
+        check_codes(beside, beside_scales, whole, x.double(), 0.0)
+        assert torch.equal(codes, beside) and torch.equal(scales, beside_scales)
+        gate_up = normal(rows, 2 * width, seed=76).to(DT[dtype])
+        ops().swiglu_int8(codes, scales, gate_up)
+        ops().swiglu_int8(beside, beside_scales, gate_up)
+        check_codes(beside, beside_scales, whole, gate_formula(gate_up, "silu"), 2.0 ** -15)
+        assert torch.equal(codes, beside) and torch.equal(scales, beside_scales)
+        assert bool((buffer[:shift] == 99).all()) and bool((buffer[shift + rows * width:] == 99).all())
+
+
 @pytest.mark.parametrize("add", [None, "float32", "bfloat16"])
 @pytest.mark.parametrize("rows,width", [(2000, 5124), (1800, 5122), (1200, 8192), (1300, 10244), (1301, 12300)])
 def test_many_long_norms(rows, width, add):

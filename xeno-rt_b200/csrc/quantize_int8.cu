@@ -19,7 +19,8 @@
 // one store.  Measured on a B200, operands from memory, microseconds (bytes that it cannot do without at 6.55 TB/s): norm after
 // an addition of 1 row of 4,096 2.2, of 2,048 16.3 (14.1), of 8,191 of 5,120, float32 79-86 (83); gate of 8 rows of 14,336
 // units 2.8, of 2,048 29.6 (22.4), of 2,000 of 25,600 51 (39); plain rows, 64 of 4,096 1.5, 4,096 of 8,192 20.7 (15.4).
-// Rows of a width or an address that allows single values only take longer: norm of 2,047 of 4,095 37 (16.6).
+// Rows of a width or an address that allows single values only take longer: norm of 2,047 of 4,095 36 (16.6), gates of 2,000 of
+// 25,599 75 (39).
 #include <stddef.h>
 
 #include <type_traits>
@@ -335,7 +336,7 @@ __device__ __forceinline__ RowScaleOf scale_of(const ROWS& rows, int width, uint
   s.inverse = 1.0f / s.scale;
   return s;
 }
-template <class ROWS, int VEC, int ITEMS>
+template <class ROWS, int VEC, int ITEMS, bool LOOSE = false>
 __device__ __forceinline__ void finish_row(int8_t* codes, float* scales, const ROWS& rows, int row, int width, int ld_codes, int stride,
                                            uint32_t bits, float squares, float (&v)[ITEMS][VEC]) {
   const RowScaleOf s = scale_of(rows, width, bits, squares);
@@ -349,7 +350,15 @@ __device__ __forceinline__ void finish_row(int8_t* codes, float* scales, const R
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[i][j] *= s.factor;
       }
-      store_codes<VEC, ROWS::EXACT>(dst + c, v[i], s.scale, s.inverse, s.broken);
+      if (LOOSE && c + VEC > width) {  // the row's last elements, one by one
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float one[1] = {v[i][j]};
+          store_codes<1, ROWS::EXACT>(dst + width - VEC + j, one, s.scale, s.inverse, s.broken);
+        }
+      } else {
+        store_codes<VEC, ROWS::EXACT>(dst + c, v[i], s.scale, s.inverse, s.broken);
+      }
     }
   }
 }
@@ -485,19 +494,26 @@ __device__ __forceinline__ void ring_edges(const ROWS& rows, int row, int width,
     reinterpret_cast<T*>(place + (copy.begin & 15))[i] = reinterpret_cast<const T*>(copy.begin)[i];
 }
 
-// A row's elements in its stage.
-template <class ROWS>
+// A row's elements in its stage.  LOOSE: pieces begin at any element, and are read one by one.
+template <class ROWS, bool LOOSE>
 struct RingRow {
   const unsigned char* first;
   const unsigned char* second;  // of the streams: the places of element 0
   template <int I, int VEC>
   __device__ __forceinline__ void operator()(int c, float (&v)[VEC]) const {
-    load_some<VEC>(reinterpret_cast<const typename ROWS::template From<I>*>(I == 0 ? first : second) + c, v);
+    const auto* from = reinterpret_cast<const typename ROWS::template From<I>*>(I == 0 ? first : second) + c;
+    if constexpr (LOOSE) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = to_float(from[j]);
+    } else {
+      load_some<VEC>(from, v);
+    }
   }
 };
 
-// Rows blockIdx.x, blockIdx.x + gridDim.x, ..
-template <class ROWS, int VEC, int ITEMS>
+// Rows blockIdx.x, blockIdx.x + gridDim.x, ..  LOOSE: rows whose width or address allows no pieces of VEC in memory, whose codes'
+// addresses do: the last piece is the row's last VEC elements then, some of them for the second time.
+template <class ROWS, int VEC, int ITEMS, bool LOOSE>
 __global__ void __launch_bounds__(ring_threads(VEC * ITEMS))
 quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROWS rows, int n, int width, int ld_codes, int stages,
                           int* error_flag) {
@@ -557,7 +573,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
       if (error_flag != nullptr) atomicExch(error_flag, 7);
     }
     const unsigned char* place = ring + s * stage_bytes;
-    RingRow<ROWS> from{place, place + room0};
+    RingRow<ROWS, LOOSE> from{place, place + room0};
     if constexpr (VEC < 8) {
       from.first += (uintptr_t)ring_source<ROWS, 0>(rows, row, width) & 15;
       if constexpr (ROWS::STREAMS == 2) from.second += (uintptr_t)ring_source<ROWS, 1>(rows, row, width) & 15;
@@ -593,7 +609,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
       __syncwarp();
       if (row + (long long)stages * gridDim.x < n && !given_up) fetch(row + stages * gridDim.x, s);
     }
-    finish_row<ROWS, VEC, ITEMS>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
+    finish_row<ROWS, VEC, ITEMS, LOOSE>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
     if (++s == stages) { s = 0; turn ^= 1; }
     if (given_up) {
       if (threadIdx.x == 0) mbar_wait_copies(full, stages, &abort_flag);
@@ -617,10 +633,15 @@ template <typename TA, typename TW> bool fits(const NormedRows<TA, TW>& r, int w
   return pieces_fit(r.x, width, vec) && pieces_fit(r.weight, width, vec) && pieces_fit(r.add, width, vec) && pieces_fit(r.sum, width, vec);
 }
 
-template <class ROWS, int VEC, int PER>
+template <class ROWS, int VEC, int PER, bool LOOSE = false>
 int launch_quantize_ring(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag,
                          cudaStream_t stream, bool& taken) {
-  constexpr auto kernel = quantize_int8_ring_kernel<ROWS, VEC, PER / VEC>;
+  // Single values, but codes that allow pieces of four: four neighbours a thread, read one by one.  Microseconds, so / single
+  // values: 2,000 gates of 25,599 units 75 / 208, 600 of 5,003 7.9 / 13.2; 4,000 plain rows of 4,001 17.6 / 26.4.
+  if constexpr (VEC == 1 && !ROWS::NORMED)
+    if (((uintptr_t)codes | (uintptr_t)ld_codes) % 4 == 0)
+      return launch_quantize_ring<ROWS, 4, PER, true>(codes, scales, rows, n, width, ld_codes, error_flag, stream, taken);
+  constexpr auto kernel = quantize_int8_ring_kernel<ROWS, VEC, PER / VEC, LOOSE>;
   const int threads = ((width + PER - 1) / PER + 31) / 32 * 32, stage = ring_stage<ROWS>(width), room = 208 * 1024;
   if (threads > ring_threads(PER)) return XRT_OK;
   int blocks = ring_threads(PER) / threads < 8 ? ring_threads(PER) / threads : 8;

@@ -170,7 +170,7 @@ struct PlainRows {
   __device__ __forceinline__ void wait() { pdl_wait(x); }
   // the values from a row's streams where those lie in shared memory
   template <int VEC, class READ> __device__ __forceinline__ void read(int c, int, const READ& get, float (&v)[VEC]) const { get.template operator()<0, VEC>(c, v); }
-  template <int VEC> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
+  template <int VEC, bool LOOSE = false> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
   template <int VEC, bool AGAIN> __device__ __forceinline__ void load(int row, int c, int width, float (&v)[VEC]) const {
     load_some<VEC>(x + (size_t)row * width + c, v);
   }
@@ -233,7 +233,7 @@ struct GatedRows {
     get.template operator()<0, VEC>(width + c, u);
     gated<VEC>(v, u, c);
   }
-  template <int VEC> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
+  template <int VEC, bool LOOSE = false> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
   template <int VEC, bool AGAIN> __device__ __forceinline__ void load(int row, int c, int width, float (&v)[VEC]) const {
     const T* p = gate_up + (size_t)row * 2 * width + c;
     float u[VEC];
@@ -276,8 +276,15 @@ struct NormedRows {
   float eps;
   int early;  // the weight may be read before the kernel before this one is done
   __device__ __forceinline__ void wait() { pdl_wait(x, add); }
-  template <int VEC> __device__ __forceinline__ void ahead(int c, int width, float (&w)[VEC]) const {
-    if (c < width) load_some<VEC>(weight + c, w);
+  // LOOSE: pieces begin at any element, the last one with the row's last VEC elements
+  template <int VEC, bool LOOSE = false> __device__ __forceinline__ void ahead(int c, int width, float (&w)[VEC]) const {
+    if (c >= width) return;
+    if constexpr (LOOSE) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[i] = to_float(weight[min(c, width - VEC) + i]);
+    } else {
+      load_some<VEC>(weight + c, w);
+    }
   }
   template <int VEC, bool AGAIN> __device__ __forceinline__ void load(int row, int c, int width, float (&v)[VEC]) const {
     const size_t at = (size_t)row * width + c;
@@ -293,12 +300,14 @@ struct NormedRows {
       }
     }
   }
-  template <int VEC, bool AGAIN>
+  template <int VEC, bool AGAIN, bool LOOSE = false>
   __device__ __forceinline__ void settle(int row, int c, int width, const float (&w)[VEC], float (&v)[VEC], float& squares) const {
+    static_assert(!LOOSE || !ADDS, "a sum's pieces would be written in parts of the memory's 32 bytes");
     if constexpr (ADDS && !AGAIN) store_some<VEC>(sum + (size_t)row * width + c, v);
+    const int first = LOOSE ? min(c, width - VEC) : c;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      squares = fmaf(v[i], v[i], squares);
+      if (!LOOSE || first + i >= c) squares = fmaf(v[i], v[i], squares);  // (what lies before belongs to another piece too)
       v[i] *= w[i];
     }
   }
@@ -538,7 +547,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
   auto keep = [&]() {
     if constexpr (KEEPS) {
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) rows.template ahead<VEC>((int)threadIdx.x * VEC + i * stride, width, kept[i]);
+      for (int i = 0; i < ITEMS; ++i) rows.template ahead<VEC, LOOSE>((int)threadIdx.x * VEC + i * stride, width, kept[i]);
     }
   };
   if (rows.early) keep();
@@ -591,11 +600,11 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
       const int c = (int)threadIdx.x * VEC + i * stride;
       if (!ROWS::NORMED || c < width) {
         if constexpr (KEEPS) {
-          rows.template settle<VEC, false>(row, c, width, kept[i], v[i], squares);
+          rows.template settle<VEC, false, LOOSE>(row, c, width, kept[i], v[i], squares);
         } else if constexpr (ROWS::NORMED) {
           float w[VEC];
-          rows.template ahead<VEC>(c, width, w);
-          rows.template settle<VEC, false>(row, c, width, w, v[i], squares);
+          rows.template ahead<VEC, LOOSE>(c, width, w);
+          rows.template settle<VEC, false, LOOSE>(row, c, width, w, v[i], squares);
         }
         most_here = largest_of<VEC>(most_here, v[i]);
       }
@@ -637,8 +646,10 @@ template <class ROWS, int VEC, int PER, bool LOOSE = false>
 int launch_quantize_ring(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag,
                          cudaStream_t stream, bool& taken) {
   // Single values, but codes that allow pieces of four: four neighbours a thread, read one by one.  Microseconds, so / single
-  // values: 2,000 gates of 25,599 units 75 / 208, 600 of 5,003 7.9 / 13.2; 4,000 plain rows of 4,001 17.6 / 26.4.
-  if constexpr (VEC == 1 && !ROWS::NORMED)
+  // values: 2,000 gates of 25,599 units 75 / 208, 600 of 5,003 7.9 / 13.2; 4,000 plain rows of 4,001 17.6 / 26.4;
+  // 2,047 norms of 4,095 16.5 / 18.6.  With an addition (whose sums would be written in parts of 32 bytes) 8,191 of 4,097 185 / 119, and
+  // single values stay.
+  if constexpr (VEC == 1 && ROWS::STREAMS == 1)
     if (((uintptr_t)codes | (uintptr_t)ld_codes) % 4 == 0)
       return launch_quantize_ring<ROWS, 4, PER, true>(codes, scales, rows, n, width, ld_codes, error_flag, stream, taken);
   constexpr auto kernel = quantize_int8_ring_kernel<ROWS, VEC, PER / VEC, LOOSE>;

@@ -216,6 +216,17 @@ def test_gate_options(width, kind):
     check_codes(codes, scales, whole, gate_formula(gate_up, gate), 2.0 ** -15)
 
 
+@pytest.mark.parametrize("width", [4096, 4100, 4099, 17001])
+@pytest.mark.parametrize("kind", ["limited", "limited and biased", "biased"])
+def test_gate_options_of_many_rows(width, kind):
+    bias = normal(2 * width, seed=2) if "biased" in kind else None
+    gate = ops().Gate("gated_sigmoid", 2.0, 1.7, bias) if "limited" in kind else ops().Gate("silu", bias=bias)
+    gate_up = (normal(500, 2 * width, seed=3) * 2).bfloat16()
+    codes, scales, whole = room(500, width)
+    ops().swiglu_int8(codes, scales, gate_up, gate)
+    check_codes(codes, scales, whole, gate_formula(gate_up, gate), 2.0 ** -15)
+
+
 @pytest.mark.parametrize("add", [None, "float32", "bfloat16"])
 @pytest.mark.parametrize("w_dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("width", WIDTHS)

@@ -256,7 +256,9 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 // overlaps the predecessor's tail and hides its own launch latency; pdl_wait() returns once the
 // predecessor has completed and its writes are visible.  Every kernel of the decode step calls
 // pdl_trigger() first (its successor may be launched) and pdl_wait() before it touches anything a
-// predecessor wrote or reads anything it will overwrite.  Tuning::pdl = false turns the launch
+// predecessor wrote or reads anything it will overwrite.  A kernel that allocates tensor memory triggers only once it has it
+// (one thread of a block is enough): else a block of its successor, launched early onto the same multiprocessor, may take the
+// columns that a block before it still waits for, and keep them in its own wait for that block's kernel.  Tuning::pdl = false turns the launch
 // attribute off (the instructions are then no-ops).
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

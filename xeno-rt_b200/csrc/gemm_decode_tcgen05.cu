@@ -104,7 +104,6 @@ gemm_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   float* row_inv = reinterpret_cast<float*>(smem + (size_t)stages * stage_bytes + 512);  // [nb] when the input's norm is pending
   float* recv = reinterpret_cast<float*>(smem + (size_t)stages * stage_bytes + 1024);    // the cluster's sums for this block's rows
 
-  pdl_trigger();
   if (shape.clustered) dg_cluster_arrive();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_items = shape.tiles * shape.splits;
@@ -120,6 +119,7 @@ gemm_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(shape.tmem_cols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    pdl_trigger();  // not before: see common.cuh
   }
   fence_before();
   __syncthreads();

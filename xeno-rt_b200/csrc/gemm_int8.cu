@@ -102,7 +102,6 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles_m = (M + TILE_ROWS - 1) / TILE_ROWS, tiles_n = (N + BN - 1) / BN;
   const int n_tiles = tiles_m * tiles_n;
@@ -125,6 +124,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    pdl_trigger();  // not before: see common.cuh
   }
   fence_before();
   __syncthreads();
@@ -468,7 +468,6 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   // [split][weight row][row of codes]; where K is not split, the ring is free when the sums come
   int* recv = reinterpret_cast<int*>(splits > 1 ? tail + FEW_TAIL_BYTES : smem);
 
-  pdl_trigger();
   if (splits > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // (nothing here divides: what a block does before its first copies is a tenth of a short product)
@@ -562,6 +561,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     if (warp == FEW_PRODUCERS) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_cols));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+      pdl_trigger();  // not before: see common.cuh
     }
     fence_before();
     asm volatile("bar.sync 2, 160;" ::: "memory");  // the MMA warp and the finishing warps

@@ -1,6 +1,8 @@
 """Who may hold tensor memory while somebody else waits for it (reads the kernels' sources and plans: no GPU)."""
 import os
 import re
+import shutil
+import subprocess
 
 import pytest
 
@@ -24,3 +26,60 @@ def test_a_successor_may_be_launched_only_when_the_columns_are_taken(body):
     triggers = [m.start() for m in re.finditer(r"pdl_trigger\(\)", body)]
     allocations = [m.start() for m in re.finditer(r"tcgen05\.alloc\.", body)]
     assert not triggers or min(triggers) > max(allocations)
+
+
+def test_blocks_that_fit_a_multiprocessor_find_their_columns():
+    """The 8-bit products of few rows: shared memory in proportion to the columns, for a device of 148 multiprocessors."""
+    from xeno_rt_b200.core import KernelError
+    from xeno_rt_b200.csrc import ops
+    try:
+        ops.library()  # the arithmetic lives beside the kernel it describes; building needs nvcc, not a GPU
+    except KernelError as exc:
+        pytest.skip(f"the kernel library cannot be built here: {exc}")
+    seen = set()
+    for m in (1, 16, 17, 33, 48, 49, 64, 65, 80, 96, 97, 112, 128):
+        for n in (1, 32, 72, 515, 1024, 2048, 4096, 6144, 10240, 19000, 28672, 51200, 102400):
+            for k in (1, 128, 129, 300, 512, 1000, 1024, 2048, 4096, 14336, 131071):
+                plan = ops.gemm_int8_plan(148, m, n, k)
+                if plan.kernel == "few":
+                    seen.add((plan.columns, plan.splits))
+                    assert (plan.shared_bytes + 1024) * 512 >= plan.columns * 228 * 1024
+                    assert plan.shared_bytes <= 227 * 1024
+    assert {columns for columns, _ in seen} == {32, 64, 128, 256} and {splits for _, splits in seen} == {1, 2, 3, 4}
+
+
+_DECODE = r"""
+#include <cuda_runtime.h>
+#include <cstdio>
+inline cudaError_t no_device(int*) { return cudaErrorNoDevice; }
+#define cudaGetDevice no_device
+#include "gemm_decode_tcgen05.cu"
+namespace xrt { const Tuning& tuning() { static const Tuning t; return t; } }
+int main() {
+  int bad = 0, most = 0, plans = 0;
+  for (int mode = 0; mode < 3; ++mode)
+    for (int m = 1; m <= 128; m += m < 16 ? 5 : 16)
+      for (int n : {128, 1000, 4096, 14336, 28672, 128256})
+        for (int k : {64, 512, 4096, 14336}) {
+          xrt::DecodeGemmShape shape;
+          int smem = 0, blocks = 0;
+          if (xrt::plan_decode_gemm(m, n, k, n, mode, mode == 2 ? n : 0, 148, &shape, &smem, &blocks) != XRT_OK) continue;
+          ++plans;
+          if (shape.tmem_cols > most) most = shape.tmem_cols;
+          if ((smem + 1024) * 512ll < shape.tmem_cols * 228ll * 1024 || smem > 227 * 1024) ++bad;
+        }
+  printf("%d %d %d", plans, bad, most);
+  return 0;
+}
+"""
+
+
+def test_the_same_of_the_products_of_few_rows_in_bfloat16(tmp_path):
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no nvcc")
+    (tmp_path / "main.cu").write_text(_DECODE)
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O0", "-Xcicc", "-O0", "-Xptxas", "-O0", "-std=c++17", "-I", CSRC,
+                    "-o", str(tmp_path / "main"), str(tmp_path / "main.cu")], check=True, capture_output=True, text=True)
+    plans, bad, most = map(int, subprocess.run([str(tmp_path / "main")], check=True, capture_output=True, text=True).stdout.split())
+    assert plans > 200 and most == 512 and bad == 0

@@ -769,6 +769,7 @@ static int plan_decode_gemm(int M, int N, int K, int ldo, int mode, int up_rows,
   shape.tmem_cols = cols;
   shape.clustered = 0;
   *smem_out = shape.stages * stage_bytes + 1024 + recv_bytes + 1024;
+  if (*smem_out < shared_bytes_of_columns(cols)) *smem_out = shared_bytes_of_columns(cols);
   const int items = shape.tiles * shape.splits;
   *blocks_out = items < sm_count ? items : sm_count;
   *shape_out = shape;

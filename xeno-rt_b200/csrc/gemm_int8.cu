@@ -431,6 +431,11 @@ struct FewShape {
   int early;     // the weight may be read before the kernel before this one is done
 };
 
+__host__ __device__ inline int few_columns(const FewShape& s) {  // of tensor memory
+  int columns = 32;
+  while (columns < (s.rows > 128 ? 2 : 1) * s.nb) columns *= 2;
+  return columns;
+}
 __host__ __device__ inline int few_w_bytes(const FewShape& s) { return (s.rows * I8_BK + 1023) & ~1023; }  // of a slab
 __host__ __device__ inline int few_stage_bytes(const FewShape& s) { return s.slabs * (few_w_bytes(s) + s.nb * I8_BK); }
 // Weight rows that one block of a cluster finishes; the last has the remainder.
@@ -473,9 +478,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   // (nothing here divides: what a block does before its first copies is a tenth of a short product)
   const int tile = (int)blockIdx.y, split = (int)blockIdx.x;
   const int kb0 = shape.k_each * split + min(split, shape.k_more), kb1 = kb0 + shape.k_each + (split < shape.k_more ? 1 : 0);
-  const int groups = shape.rows > 128 ? 2 : 1;
-  int tmem_cols = 32;
-  while (tmem_cols < groups * nb) tmem_cols *= 2;
+  const int groups = shape.rows > 128 ? 2 : 1, tmem_cols = few_columns(shape);
   const int per = few_rows_per_block(shape), recv_row = few_recv_row(shape);
 
   if (warp == 0) {
@@ -691,7 +694,9 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 }
 
 static int few_shared_bytes(const FewShape& s) {
-  return few_ring_bytes(s) + FEW_TAIL_BYTES + (s.splits > 1 ? few_recv_bytes(s) : 0) + 1024;
+  const int bytes = few_ring_bytes(s) + FEW_TAIL_BYTES + (s.splits > 1 ? few_recv_bytes(s) : 0) + 1024;
+  const int least = shared_bytes_of_columns(few_columns(s));  // (two blocks a multiprocessor at most take half of it each)
+  return bytes > least ? bytes : least;
 }
 
 // The tile, the parts of K and the ring of a product, from what was measured on a B200 (148 multiprocessors).
@@ -836,6 +841,46 @@ struct XrtInt8Call {
 };
 static_assert(offsetof(XrtInt8Call, M) == 56 && offsetof(XrtInt8Call, constant_weight) == 88, "seven pointers, then nine ints");
 
+namespace xrt {
+
+// The kernel that takes a product: the few rows' with `shape`, or tiles of `tiles.form`.
+struct Int8Choice {
+  bool few;
+  FewShape shape;
+  Int8Form tiles;
+};
+static Int8Choice int8_choice(const Int8Product& p) {
+  // (The few rows' kernel: its tiles, of 64 weight rows at least, are a grid's second dimension.)
+  Int8Choice c = {p.M <= FEW_MAX_ROWS && p.N <= 65535 * 64, {}, {0, 0}};
+  if (c.few) c.shape = few_shape(p);
+  const bool either = c.few && p.M > ((p.N + c.shape.rows - 1) / c.shape.rows * c.shape.splits > p.sm_count ? 16 : 48);
+  if (!c.few || either) c.tiles = int8_form(p);
+  if (either) c.few = few_us(c.shape, p.K, p.sm_count) <= c.tiles.us;
+  return c;
+}
+
+}  // namespace xrt
+
+// What the launcher would do with a product on a device of `sm_count` multiprocessors (host arithmetic): plan[0] = 0 to 3 the tile
+// (int8_form), 4 the few rows' kernel; and of that one plan[1] = weight rows of a tile, plan[2] = parts of K, plan[3] = blocks,
+// plan[4] = bytes of shared memory a block, plan[5] = columns of tensor memory a block (zeros for tiles).
+XRT_EXPORT int xrt_gemm_int8_plan(int M, int N, int K, int sm_count, int* plan) {
+  if (M <= 0 || N <= 0 || K <= 0 || sm_count <= 1 || plan == nullptr) return XRT_ERR_ARGUMENT;
+  xrt::Int8Product p = {};
+  p.M = M; p.N = N; p.K = K; p.sm_count = sm_count;
+  const xrt::Int8Choice c = xrt::int8_choice(p);
+  for (int i = 0; i < 6; ++i) plan[i] = 0;
+  plan[0] = c.few ? 4 : c.tiles.form;
+  if (c.few) {
+    plan[1] = c.shape.rows;
+    plan[2] = c.shape.splits;
+    plan[3] = (N + c.shape.rows - 1) / c.shape.rows * c.shape.splits;
+    plan[4] = xrt::few_shared_bytes(c.shape);
+    plan[5] = xrt::few_columns(c.shape);
+  }
+  return XRT_OK;
+}
+
 XRT_EXPORT int xrt_gemm_int8(const XrtInt8Call* call, cudaStream_t stream) {
   const XrtInt8Call& c = *call;
   if (c.M < 0 || c.N <= 0 || c.K <= 0 || c.K > 131071 || c.ldx < c.K || c.ldw < c.K || c.ldo < c.N || c.mode < 0 || c.mode > 1)
@@ -846,19 +891,12 @@ XRT_EXPORT int xrt_gemm_int8(const XrtInt8Call* call, cudaStream_t stream) {
   const xrt::Int8Product p{c.out, c.codes, c.w, c.M, c.N, c.K, c.ldx, c.ldw, c.ldo, {c.scales, c.w_scales, c.bias},
                            xrt::multiprocessors(), c.error_flag};
   if (p.sm_count <= 1) return XRT_ERR_UNSUPPORTED;
-  // (The few rows' kernel: its tiles, of 64 weight rows at least, are a grid's second dimension.)
-  xrt::FewShape shape = {};
-  xrt::Int8Form tiles = {0, 0};
-  bool few = c.M <= xrt::FEW_MAX_ROWS && c.N <= 65535 * 64;
-  if (few) shape = xrt::few_shape(p);
-  const bool either = few && c.M > ((c.N + shape.rows - 1) / shape.rows * shape.splits > p.sm_count ? 16 : 48);
-  if (!few || either) tiles = xrt::int8_form(p);
-  if (either) few = xrt::few_us(shape, c.K, p.sm_count) <= tiles.us;
+  const xrt::Int8Choice choice = xrt::int8_choice(p);
   if (c.mode == 1)
-    return few ? xrt::launch_gemm_int8_few<1, float>(p, shape, c.constant_weight, stream)
-               : xrt::launch_gemm_int8<1, float>(p, tiles.form, stream);
+    return choice.few ? xrt::launch_gemm_int8_few<1, float>(p, choice.shape, c.constant_weight, stream)
+                      : xrt::launch_gemm_int8<1, float>(p, choice.tiles.form, stream);
   XRT_DISPATCH_DTYPE(c.out_dtype, TO, {
-    return few ? xrt::launch_gemm_int8_few<0, TO>(p, shape, c.constant_weight, stream)
-               : xrt::launch_gemm_int8<0, TO>(p, tiles.form, stream);
+    return choice.few ? xrt::launch_gemm_int8_few<0, TO>(p, choice.shape, c.constant_weight, stream)
+                      : xrt::launch_gemm_int8<0, TO>(p, choice.tiles.form, stream);
   });
 }

@@ -97,6 +97,7 @@ _SIGNATURES = {
     "xrt_swiglu_int8": [_P, _P],
     "xrt_rmsnorm_int8": [_P, _P],
     "xrt_gemm_int8": [_P, _P],
+    "xrt_gemm_int8_plan": [_I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)],
     "xrt_fill_normal": [_P, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_double, _I, _P],
     "xrt_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P],
     "xrt_mark_seen": [_P, _I, _P, _P, _I, _I, _P],
@@ -1870,3 +1871,23 @@ def gemm_int8(out, codes, scales, weight, weight_scales, accumulate: bool = Fals
         0 if bias is None else _vector(bias, "bias", what, n), _error_flag_pointer(out.get_device()), m, n, k, ldx, ldw,
         ldo if m > 1 else n, _code(out.dtype), 1 if accumulate else 0, 1 if constant_weight else 0)
     _run_int8(what, (out, codes, scales, weight, weight_scales, bias), _kernels().xrt_gemm_int8, call)
+
+
+@dataclasses.dataclass(frozen=True)
+class Int8Plan:
+    """What ``gemm_int8`` does with a product: ``kernel`` "few" or the tile it walks; of "few" the weight rows of a tile, the parts
+    of K, the blocks, and a block's bytes of shared memory and columns of tensor memory (0 else)."""
+    kernel: str
+    rows: int
+    splits: int
+    blocks: int
+    shared_bytes: int
+    columns: int
+
+
+def gemm_int8_plan(sms: int, m: int, n: int, k: int) -> Int8Plan:
+    """The plan of ``gemm_int8`` for [m, k] codes and [n, k] weights on a device of ``sms`` multiprocessors.  Host arithmetic
+    only: no device is needed."""
+    plan = (ctypes.c_int * 6)()
+    _check(library().xrt_gemm_int8_plan(m, n, k, sms, plan), "gemm_int8_plan")
+    return Int8Plan(("pair256", "pair128", "single256", "single128", "few")[plan[0]], *plan[1:])

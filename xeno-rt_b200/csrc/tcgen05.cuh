@@ -15,6 +15,13 @@ namespace sm100 {
 
 constexpr long long SPIN_LIMIT = 1ll << 24;  // polls of a barrier before a wait gives up
 
+// The shared memory, in bytes, that a block which allocates `columns` of tensor memory must at least be launched with where it is part of
+// a cluster.  An allocation waits until the multiprocessor has the columns to spare.  Two clusters that run at the same
+// time, each with one block that has its columns and one that waits for those which the other holds, would wait for ever.  So
+// columns are given out with shared memory: 456 of a multiprocessor's 233,472 bytes (1,024 of every block's share are the
+// system's) for each of its 512 columns, and blocks that fit one multiprocessor together always find theirs.
+__host__ __device__ constexpr int shared_bytes_of_columns(int columns) { return columns * 456 - 1024; }
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // One lane of a warp whose lanes are all here.  The compiler knows it for one lane, and so that the operands of what it issues are

@@ -270,21 +270,23 @@ gemm_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
     const int r = quarter * 32 + lane;  // weight row inside the tile = TMEM lane
     int item_i = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++item_i) {
+    for (int item = blockIdx.x; item < n_items; item += gridDim.x, ++item_i) {
       const int tile = item / shape.splits, split = item % shape.splits;
       const int kb0 = split * shape.k_per_split;
-      const bool has_k = kb0 < k_iters_total;  // a split beyond K (uneven division) contributes zeros
+      // A split beyond K (uneven division) contributes zeros; so does all that a warp would take after a wait of its own
+      // ran out: it says so at once and goes on, since the other warps may still come to the barriers below.
+      bool has_k = kb0 < k_iters_total && ok;
       const int a = item_i & 1;
       const int n = tile * DG_ROWS + r;  // output column = weight row
       const uint32_t tmem_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + a * acc_cols;
       if (has_k) {
-        ok = mbar_wait(smem_u32(&acc_full[a]), (item_i >> 1) & 1, abort_flag);
-        if (!ok) break;
+        ok = has_k = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[a]), (item_i >> 1) & 1, abort_flag));
+        if (!ok && lane == 0) { *abort_flag = 1; if (error_flag != nullptr) atomicExch(error_flag, 4); }
         fence_after();
       }
       if (shape.splits == 1) {
         // one split: straight to the output
-        for (int c = 0; c < shape.nb; c += 16) {
+        for (int c = 0; ok && c < shape.nb; c += 16) {
           uint32_t v[16], u[16];
           tmem_ld16(v, tmem_row + c);
           if (MODE == 2) tmem_ld16(u, tmem_row + shape.nb + c);
@@ -413,7 +415,6 @@ gemm_decode_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         asm volatile("bar.sync 1, 128;" ::: "memory");  // last_flag is rewritten for the next item
       }
     }
-    if (!ok && lane == 0) { *abort_flag = 1; if (error_flag != nullptr) atomicExch(error_flag, 4); }
   }
 
   if (shape.clustered) {

@@ -232,8 +232,14 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         by_column[BN + i] = scales.bias != nullptr ? scales.bias[n] : 0.f;
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");  // (the set of the tile before last is not read any more)
-      ok = mbar_wait(smem_u32(&acc_full[a]), acc_turn, abort_flag);
-      if (!ok) break;
+      // A warp whose wait ran out says so at once, and from then on only meets the others at this barrier, which they may
+      // still come to.
+      if (!ok) continue;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[a]), acc_turn, abort_flag));
+      if (!ok) {
+        if (lane == 0) give_up();
+        continue;
+      }
       fence_after();
       const uint32_t tmem_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + a * BN;
 #pragma unroll 1
@@ -301,7 +307,6 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       if (++a == 2) { a = 0; acc_turn ^= 1; }
     }
     tma_stores_done();
-    if (!ok && lane == 0) give_up();
   }
 
   fence_before();

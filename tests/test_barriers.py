@@ -46,3 +46,12 @@ def test_no_warp_leaves_a_loop_in_which_others_wait_for_it(header, body):
 
 def test_there_are_such_loops():
     assert {p.id.split(":")[0] for p in _loops_with_a_named_barrier()} >= {"gemm_int8.cu", "gemm_decode_tcgen05.cu"}
+
+
+def test_the_last_wait_for_copies_has_a_bound_of_its_own():
+    """It runs only where the abort flag is raised: a wait that looked at the flag would end with copies still in flight."""
+    with open(os.path.join(CSRC, "tcgen05.cuh")) as fh:
+        text = fh.read()
+    at = text.index("void mbar_wait_copies(")
+    function = text[at:_closing(text, text.index("{", at), "{}")]
+    assert "COPY_LIMIT" in function and "abort_flag" not in function and "mbar_wait(" not in function

@@ -311,7 +311,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 
   fence_before();
   __syncthreads();
-  if (*abort_flag && rank == 0 && threadIdx.x == 0) mbar_wait_copies(full, STAGES, abort_flag);  // (a pair's copies: all of them)
+  if (*abort_flag && rank == 0 && threadIdx.x == 0) mbar_wait_copies(full, STAGES);  // (a pair's copies: all of them)
   if (PAIR) cluster_sync();  // neither block leaves while the other may still arrive on its barriers or read its shared memory
   if (warp == 2) {
     fence_after();
@@ -691,7 +691,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     }
   }
   __syncthreads();
-  if (*abort_flag && threadIdx.x == 0) mbar_wait_copies(full, stages, abort_flag);
+  if (*abort_flag && threadIdx.x == 0) mbar_wait_copies(full, stages);
   if (warp == FEW_PRODUCERS) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols));

@@ -621,7 +621,7 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
     finish_row<ROWS, VEC, ITEMS, LOOSE>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
     if (++s == stages) { s = 0; turn ^= 1; }
     if (given_up) {
-      if (threadIdx.x == 0) mbar_wait_copies(full, stages, &abort_flag);
+      if (threadIdx.x == 0) mbar_wait_copies(full, stages);
       break;
     }
   }

@@ -13,7 +13,9 @@
 namespace xrt {
 namespace sm100 {
 
-constexpr long long SPIN_LIMIT = 1ll << 24;  // polls of a barrier before a wait gives up
+// Polls of a barrier before a wait gives up: 23 seconds (a poll of a barrier that does not complete takes 1.36 microseconds).
+constexpr long long SPIN_LIMIT = 1ll << 24;
+constexpr int COPY_LIMIT = 1 << 14;  // 22 milliseconds: thousands of times what a copy takes
 
 // The shared memory, in bytes, that a block which allocates `columns` of tensor memory must at least be launched with where it is part of
 // a cluster.  An allocation waits until the multiprocessor has the columns to spare.  Two clusters that run at the same
@@ -50,21 +52,25 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 // Bounded wait for the phase of the given parity.  False if it ran out or another role of the block
 // raised `abort_flag` (looked at every 1,024 polls): the caller leaves its loop, raises the flag and the
 // kernel's error flag; nobody spins for ever.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   for (long long spin = 0; spin < SPIN_LIMIT; ++spin) {
-    uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    if (done) return true;
+    if (mbar_poll(bar, parity)) return true;
     if ((spin & 1023) == 1023 && *abort_flag) return false;
   }
   return false;
 }
 // What a block does whose `abort_flag` is raised, before it leaves: waits until the copies that it has asked for have landed in its
-// shared memory, on the barriers that hear of them, whatever phase each is in (a phase with nothing to come runs out after
-// 1,024 polls).  For one thread.
-__device__ __forceinline__ void mbar_wait_copies(uint64_t* full, int count, volatile int* abort_flag) {
-  for (int s = 0; s < 2 * count; ++s) mbar_wait(smem_u32(&full[s >> 1]), s & 1, abort_flag);
+// shared memory, on the barriers that hear of them, whatever phase each is in (a phase that nobody completes any more runs out
+// after COPY_LIMIT polls).  For one thread.
+__device__ __forceinline__ void mbar_wait_copies(uint64_t* full, int count) {
+  for (int s = 0; s < 2 * count; ++s)
+    for (int spin = 0; spin < COPY_LIMIT && !mbar_poll(smem_u32(&full[s >> 1]), s & 1); ++spin) {}
 }
 // A tile of a two-dimensional tensor map into shared memory; c0 is the innermost coordinate (its
 // byte offset must be a multiple of 16).  No multicast: the tile goes to this block only.

@@ -21,6 +21,10 @@
 #define XRT_ERR_ARGUMENT -1
 #define XRT_ERR_UNSUPPORTED -2
 
+// The most rows, or elements of a row, of the 8-bit operators: counters of 32 bits go up to 8,192 (a block's threads times eight)
+// beyond the last one.
+#define XRT_INT8_MAX_SIZE (0x7fffffff - 8191)
+
 #define XRT_EXPORT extern "C" __attribute__((visibility("default")))
 
 namespace xrt {

@@ -870,7 +870,8 @@ static Int8Choice int8_choice(const Int8Product& p) {
 // (int8_form), 4 the few rows' kernel; and of that one plan[1] = weight rows of a tile, plan[2] = parts of K, plan[3] = blocks,
 // plan[4] = bytes of shared memory a block, plan[5] = columns of tensor memory a block (zeros for tiles).
 XRT_EXPORT int xrt_gemm_int8_plan(int M, int N, int K, int sm_count, int* plan) {
-  if (M <= 0 || N <= 0 || K <= 0 || sm_count <= 1 || plan == nullptr) return XRT_ERR_ARGUMENT;
+  if (M <= 0 || M > XRT_INT8_MAX_SIZE || N <= 0 || N > XRT_INT8_MAX_SIZE || K <= 0 || K > 131071 || sm_count <= 1 || plan == nullptr)
+    return XRT_ERR_ARGUMENT;
   xrt::Int8Product p = {};
   p.M = M; p.N = N; p.K = K; p.sm_count = sm_count;
   const xrt::Int8Choice c = xrt::int8_choice(p);
@@ -890,6 +891,7 @@ XRT_EXPORT int xrt_gemm_int8(const XrtInt8Call* call, cudaStream_t stream) {
   const XrtInt8Call& c = *call;
   if (c.M < 0 || c.N <= 0 || c.K <= 0 || c.K > 131071 || c.ldx < c.K || c.ldw < c.K || c.ldo < c.N || c.mode < 0 || c.mode > 1)
     return XRT_ERR_ARGUMENT;
+  if (c.M > XRT_INT8_MAX_SIZE || c.N > XRT_INT8_MAX_SIZE) return XRT_ERR_ARGUMENT;
   if (c.mode == 1 && c.out_dtype != XRT_F32) return XRT_ERR_ARGUMENT;
   if (c.ldx % 16 != 0 || c.ldw % 16 != 0 || ((uintptr_t)c.codes & 15) || ((uintptr_t)c.w & 15)) return XRT_ERR_UNSUPPORTED;
   if (c.M == 0) return XRT_OK;

@@ -1704,6 +1704,7 @@ def linear_recurrence_step(out, p, w: RecurrenceWeights, state, ring, tok_slot, 
 
 # ------------------------------------------------------------------ products of 8-bit integers
 INT8_MAX_INPUTS = 131071  # 128 * 128 * K stays below 2^31
+INT8_MAX_SIZE = 2 ** 31 - 8192  # rows, and elements of a row: the kernels count them in 32 bits
 
 
 def int8_rows(rows: int, width: int, device) -> torch.Tensor:
@@ -1756,6 +1757,8 @@ def _codes(t, name: str, what: str, rows: int, width: int) -> int:
     """The distance of the rows of an int8 tensor [rows, width] in bytes."""
     if t.dtype != torch.int8 or t.shape != (rows, width):
         raise KernelError(f"{what}: {name} must be int8 [{rows}, {width}], not {t.dtype} {tuple(t.shape)}")
+    if rows > INT8_MAX_SIZE or width > INT8_MAX_SIZE:
+        raise KernelError(f"{what}: [{rows}, {width}] is too large; at most {INT8_MAX_SIZE} rows or elements of a row are taken")
     distance, step = t.stride()
     if (width > 1 and step != 1) or (rows > 1 and not width <= distance < 1 << 31):
         raise KernelError(f"{what}: the rows of {name} must be contiguous and less than 2^31 bytes apart")
@@ -1781,7 +1784,7 @@ def quantize_rows(codes, scales, x) -> None:
     """Every row of ``x`` (float32 or bfloat16 [n, width]) as 8-bit integers with one scale: scales[r] = max(max |x[r]| / 127,
     2^-126), codes[r] = x[r] / scales[r] rounded to the nearest (ties to even).  ``codes`` int8 [n, width], rows contiguous
     (``int8_rows`` makes one that ``gemm_int8`` takes); ``scales`` float32 [n].  A row with a NaN or an infinity
-    gets codes 0 and the scale NaN."""
+    gets codes 0 and the scale NaN.  At most ``INT8_MAX_SIZE`` rows, and elements of a row."""
     what = "quantize_rows"
     if x.dim() != 2:
         raise KernelError(f"{what}: x must be [rows, width]")

@@ -695,7 +695,7 @@ int launch_quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int w
 // Pieces of eight, four or one value at a time: the most that rows of this width and these addresses allow.
 template <class ROWS>
 int quantize(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag, cudaStream_t stream) {
-  if (n < 0 || width <= 0 || ld_codes < width) return XRT_ERR_ARGUMENT;
+  if (n < 0 || n > XRT_INT8_MAX_SIZE || width <= 0 || width > XRT_INT8_MAX_SIZE || ld_codes < width) return XRT_ERR_ARGUMENT;
   if (n == 0) return XRT_OK;
   auto whole = [&](int vec) {
     return width % vec == 0 && fits(rows, width, vec) && ((uintptr_t)codes | (uintptr_t)ld_codes) % vec == 0;

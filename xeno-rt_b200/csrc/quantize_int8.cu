@@ -191,12 +191,14 @@ struct GatedRows {
   __host__ __device__ __forceinline__ static int length(int width) { return 2 * width; }
   static constexpr int early = 0;
   __device__ __forceinline__ void wait() { pdl_wait(gate_up); }
-  // g sigmoid(a g) u as g / (1 + 2^(-a log2(e) g)) u, with the exponent -a log2(e) g given: the exponential and the reciprocal
-  // as the multiprocessor has them (2 ulp and 1; 8 bits are kept), which end at 0 and infinity as the formula does.
-  __device__ __forceinline__ static float sigmoid(float exponent) {
+  // g sigmoid(a g) u as g / (1 + 2^(-a log2(e) g)) u: the exponential and the reciprocal as the multiprocessor has them (2 ulp and 1;
+  // 8 bits are kept).  They give 0 for results below 2^-126, but sigmoid goes on to 2^-128 before 1 + 2^x is no 32-bit number
+  // (and a gate of -88 alone in its row, times a large u, is the scale): hence 4 sigmoid, 1 / (1 / 4 + 2^(x - 2)), from x - 2,
+  // which the exponent's last addition gives.  Beyond, the result is 0, as the formula's is in 32 bits.
+  __device__ __forceinline__ static float four_sigmoid(float exponent_less_2) {
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(exponent));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(exponent_less_2));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.25f + e));
     return r;
   }
   template <int VEC> __device__ __forceinline__ void gated(float (&g)[VEC], float (&u)[VEC], int c) const {
@@ -207,7 +209,7 @@ struct GatedRows {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float x = fminf(g[i], limit);
-        g[i] = x * sigmoid(x * exponent) * (fminf(fmaxf(u[i], -limit), limit) + 1.0f);
+        g[i] = 0.25f * x * four_sigmoid(fmaf(x, exponent, -2.0f)) * (fminf(fmaxf(u[i], -limit), limit) + 1.0f);
       }
       return;
     }
@@ -215,15 +217,16 @@ struct GatedRows {
     // value is the scale
     const bool tanh_form = gate.gate_act == 1;
     if constexpr (VEC == 1) {
-      g[0] = g[0] * sigmoid(g[0] * (tanh_form ? fmaf(-GELU * 0.044715f * LOG2E, g[0] * g[0], -GELU * LOG2E) : -LOG2E)) * u[0];
+      const float by = tanh_form ? fmaf(-GELU * 0.044715f * LOG2E, g[0] * g[0], -GELU * LOG2E) : -LOG2E;
+      g[0] = 0.25f * g[0] * four_sigmoid(fmaf(g[0], by, -2.0f)) * u[0];
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; i += 2) {
         const Two x(g[i], g[i + 1]);
-        const Two exponent = x * (tanh_form ? fma_two(x * x, Two(-GELU * 0.044715f * LOG2E), Two(-GELU * LOG2E)) : Two(-LOG2E));
+        const Two by = tanh_form ? fma_two(x * x, Two(-GELU * 0.044715f * LOG2E), Two(-GELU * LOG2E)) : Two(-LOG2E);
         float first, second;
-        exponent.get(first, second);
-        (x * Two(sigmoid(first), sigmoid(second)) * Two(u[i], u[i + 1])).get(g[i], g[i + 1]);
+        fma_two(x, by, Two(-2.0f)).get(first, second);
+        (Two(0.25f) * x * Two(four_sigmoid(first), four_sigmoid(second)) * Two(u[i], u[i + 1])).get(g[i], g[i + 1]);
       }
     }
   }

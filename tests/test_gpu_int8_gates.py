@@ -71,3 +71,20 @@ def test_gates_beyond_the_last_one_are_zero():
     g = torch.full((2, 64), -120.0, device=DEV)
     codes, scales = gates(g, torch.ones_like(g), "silu")
     assert not bool(codes.any()) and bool((scales == 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,width", [(8, 7), (8, 96), (8, 5000), (8, 40000), (600, 4096), (600, 4099)])
+def test_limited_gates_that_are_no_number_break_their_row(rows, width, dtype, biased):
+    """A NaN on either side, and a gate of minus infinity (times sigmoid's 0); infinities that a limit cuts off do not."""
+    from xeno_rt_b200.csrc import ops
+    act = ops.Gate("gated_sigmoid", 2.0, 1.7, torch.zeros(2 * width, device=DEV) if biased else None)
+    gen = torch.Generator().manual_seed(2)
+    g, u = (torch.randn(rows, width, generator=gen).to(DEV).to(DT[dtype]) for _ in range(2))
+    nan, inf = float("nan"), float("inf")
+    g[0, 0], g[1, width - 1], u[2, width // 2], u[3, width - 1], g[4, 3] = nan, nan, nan, nan, -inf
+    g[5, 2], u[6, 1], u[7, width - 1] = inf, inf, -inf
+    codes, scales = gates(g, u, act)
+    assert bool(torch.isnan(scales[:5]).all()) and not bool(codes[:5].any())
+    check(codes[5:], scales[5:], formula(g[5:], u[5:], act))

@@ -201,6 +201,15 @@ struct GatedRows {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.25f + e));
     return r;
   }
+  // a limit lets what is no number through, so that its row is broken
+  __device__ __forceinline__ static float smaller(float a, float b) {
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+  }
+  __device__ __forceinline__ static float larger(float a, float b) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+  }
   template <int VEC> __device__ __forceinline__ void gated(float (&g)[VEC], float (&u)[VEC], int c) const {
     constexpr float LOG2E = 1.4426950408889634f;
     add_gate_biases<VEC, true>(g, u, c, gate);
@@ -208,8 +217,8 @@ struct GatedRows {
       const float limit = gate.gate_limit, exponent = -gate.gate_alpha * LOG2E;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float x = fminf(g[i], limit);
-        g[i] = 0.25f * x * four_sigmoid(fmaf(x, exponent, -2.0f)) * (fminf(fmaxf(u[i], -limit), limit) + 1.0f);
+        const float x = smaller(g[i], limit);
+        g[i] = 0.25f * x * four_sigmoid(fmaf(x, exponent, -2.0f)) * (smaller(larger(u[i], -limit), limit) + 1.0f);
       }
       return;
     }

@@ -37,3 +37,34 @@ def test_chains_of_short_products_on_eight_streams(m, n, k):
     ops.check_error_flag(DEV)
     for one, got in zip(want, outs):
         assert all(torch.equal(one, out) for out in got)
+
+
+@pytest.mark.parametrize("mode", ["global", "thread_local", "relaxed"])
+def test_a_first_call_inside_a_capture_reports_its_errors_too(monkeypatch, mode):
+    """The device's flag is made beside the capture: kernels of the graph get it, no replay clears it, and it is read as ever."""
+    from xeno_rt_b200.core import KernelError
+    from xeno_rt_b200.csrc import ops
+    x = torch.randn(4, 64, generator=torch.Generator().manual_seed(5)).to(DEV)
+    want, want_scales = ops.int8_rows(4, 64, DEV), torch.empty(4, device=DEV)
+    ops.quantize_rows(want, want_scales, x)
+    codes, scales = ops.int8_rows(4, 64, DEV), torch.empty(4, device=DEV)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(ops, "_error_flags", {})  # as in a process that has called nothing yet
+    monkeypatch.setattr(ops, "_error_flags_at", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode=mode):
+        ops.quantize_rows(codes, scales, x)
+        inside = ops._error_flag_pointer(0)
+    flag = ops._error_flags[0]
+    assert inside != 0 and inside == flag.data_ptr()
+    graph.replay()
+    assert torch.equal(codes, want) and torch.equal(scales, want_scales)
+    ops.check_error_flag(DEV)
+    flag.fill_(7)  # as a kernel of the graph would
+    graph.replay()
+    with pytest.raises(KernelError, match="error 7"):
+        ops.check_error_flag(DEV)
+    ops.check_error_flag(DEV)
+    del graph, codes, scales
+    torch.cuda.empty_cache()
+    assert ops.error_flag(DEV) is flag and int(flag) == 0

@@ -97,6 +97,7 @@ _SIGNATURES = {
     "xrt_swiglu_int8": [_P, _P],
     "xrt_rmsnorm_int8": [_P, _P],
     "xrt_gemm_int8": [_P, _P],
+    "xrt_exchange_capture_mode": [_I],
     "xrt_gemm_int8_plan": [_I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)],
     "xrt_fill_normal": [_P, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_double, _I, _P],
     "xrt_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P],
@@ -471,15 +472,29 @@ def gemm_reference(out, x, w, accumulate: bool = False) -> None:
 
 STREAM_MAX_ROWS = 64
 _error_flags: dict = {}
+_CAPTURE_RELAXED = 2  # cudaStreamCaptureModeRelaxed
 
 
 def error_flag(device) -> torch.Tensor:
-    """The int32 flag of ``device`` that kernels raise when a bounded wait inside them ran out.
-    Made when a model is built (never inside a stream capture)."""
+    """The int32 flag of ``device`` that kernels raise when a bounded wait inside them ran out.  Made when a model is built or at
+    the first call that needs it; inside a stream capture beside the capture, on a stream of its own, so that it is no part of
+    the graph and is cleared before the graph runs."""
     device = torch.device(device)
     key = device.index if device.index is not None else torch.cuda.current_device()
     if key not in _error_flags:
-        _error_flags[key] = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.cuda.device(key):
+            if torch.cuda.is_current_stream_capturing():
+                before = library().xrt_exchange_capture_mode(_CAPTURE_RELAXED)  # memory may be asked for beside the capture
+                try:
+                    beside = torch.cuda.Stream()
+                    with torch.cuda.stream(beside):
+                        flag = torch.zeros(1, dtype=torch.int32, device=device)
+                    beside.synchronize()
+                finally:
+                    library().xrt_exchange_capture_mode(before)
+            else:
+                flag = torch.zeros(1, dtype=torch.int32, device=device)
+            _error_flags[key] = flag
     return _error_flags[key]
 
 
@@ -1741,15 +1756,12 @@ _error_flags_at: dict = {}  # their addresses
 
 
 def _error_flag_pointer(index: int) -> int:
-    """A device's error flag for a launch; 0 (the kernel reports nothing) where it would have to be made inside a capture."""
+    """A device's error flag for a launch (0 for a tensor on none, whose call is refused)."""
     at = _error_flags_at.get(index)
     if at is None:
-        flag = _error_flags.get(index)
-        if flag is None:
-            if index < 0 or torch.cuda.is_current_stream_capturing():
-                return 0
-            flag = error_flag(torch.device("cuda", index))
-        at = _error_flags_at[index] = flag.data_ptr()
+        if index < 0:
+            return 0
+        at = _error_flags_at[index] = error_flag(torch.device("cuda", index)).data_ptr()
     return at
 
 

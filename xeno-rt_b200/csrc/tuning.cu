@@ -26,3 +26,9 @@ XRT_EXPORT int xrt_set_tuning(int key, int value) {
     default: return XRT_ERR_ARGUMENT;
   }
 }
+
+// What the calling thread may do while a stream captures (cudaStreamCaptureMode); returns the mode before, or -1.
+XRT_EXPORT int xrt_exchange_capture_mode(int mode) {
+  cudaStreamCaptureMode other = (cudaStreamCaptureMode)mode;
+  return cudaThreadExchangeStreamCaptureMode(&other) == cudaSuccess ? (int)other : -1;
+}

@@ -7,29 +7,35 @@ from __future__ import annotations
 
 import torch
 
+from ..core import KernelError
 from ..csrc import ops
 
 
 class Int8Matrix:
-    """A weight [out, in] as ``codes`` int8 and ``scales`` float32 [out]."""
+    """A weight [out, in] as ``codes`` int8 and ``scales`` float32 [out].  ``constant``: no kernel that may still run wrote the
+    codes; products of few rows then read them while the kernel before finishes."""
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
-        self.codes, self.scales = codes, scales
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, constant: bool = False):
+        self.codes, self.scales, self.constant = codes, scales, constant
 
     @classmethod
     def of(cls, weight: torch.Tensor) -> "Int8Matrix":
-        """The nearest codes of a float32 or bfloat16 weight, a scale a row."""
+        """The nearest codes of a float32 or bfloat16 weight, a scale a row.  Waits until they are written (they are constant from
+        here on), so not inside a stream capture."""
+        if weight.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise KernelError("a matrix is laid out in 8 bits outside of stream captures")
         codes = ops.int8_rows(weight.shape[0], weight.shape[1], weight.device)
         scales = torch.empty(weight.shape[0], dtype=torch.float32, device=weight.device)
         ops.quantize_rows(codes, scales, weight.contiguous())
-        return cls(codes, scales)
+        torch.cuda.current_stream(weight.device).synchronize()
+        return cls(codes, scales, constant=True)
 
     @property
     def shape(self):
         return self.codes.shape
 
     def __getitem__(self, rows: slice) -> "Int8Matrix":
-        return Int8Matrix(self.codes[rows], self.scales[rows])
+        return Int8Matrix(self.codes[rows], self.scales[rows], self.constant)
 
 
 class Int8Rows:
@@ -62,4 +68,4 @@ def product(out: torch.Tensor, x, weight: Int8Matrix, accumulate: bool) -> None:
     """out = x . weight^T, or added into a float32 ``out``; x ``Int8Rows``, or a tensor that is rounded to that first."""
     if not isinstance(x, Int8Rows):
         x = Int8Rows.of(x)
-    ops.gemm_int8(out, x.codes, x.scales, weight.codes, weight.scales, accumulate=accumulate, constant_weight=True)
+    ops.gemm_int8(out, x.codes, x.scales, weight.codes, weight.scales, accumulate=accumulate, constant_weight=weight.constant)

@@ -110,7 +110,8 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
   if (threadIdx.x == 0) {
-    // a stage is full when the producers (two, in a pair two of each block) have announced their bytes and those are there
+    // a stage is full when both operands' bytes have been announced (each by its producer, in a pair by the first block's for both
+    // blocks) and are there
     for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full[s]), 2); mbar_init(smem_u32(&empty[s]), 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(smem_u32(&acc_full[a]), 1); mbar_init(smem_u32(&acc_empty[a]), PAIR ? 256 : 128); }
     *abort_flag = 0;
@@ -765,9 +766,9 @@ static void plan_few(FewShape& s, int K, int sm_count) {
     while (s.stages > 1 && few_shared_bytes(s) > limit) --s.stages;
     if (s.stages > share) s.stages = share;
     if ((s.stages * s.slabs >= FEW_PRODUCERS || s.stages == share) && few_shared_bytes(s) <= limit) break;
+    // (this ends: all of K with one block a multiprocessor has room for four slabs of 256 weight rows and 128 rows of codes)
     if (limit == FEW_SHARED_TWO) limit = FEW_SHARED_ONE;
-    else if (s.splits > 1) --s.splits;
-    else s.rows = (s.rows / 2 + 7) / 8 * 8;  // (no product of this library's sizes comes here)
+    else --s.splits;
   }
 }
 

@@ -483,14 +483,14 @@ template <class ROWS, int I>
 __device__ __forceinline__ const typename ROWS::template From<I>* ring_source(const ROWS& rows, int row, int width) {
   return rows.template from<I>() + (size_t)row * ROWS::length(width);
 }
-// The bulk copy of a stream of a row to its place in a stage: where it begins and its bytes (0: the stream is too short for one).
+// The bulk copy of a stream of a row to its place in a stage: where the row begins, and the copy's ends.  (Rows in a ring are
+// thousands of bytes long, see ring_pays: none lies between two boundaries.)
 struct RingCopy {
   uintptr_t begin, lo, hi;
-  __device__ __forceinline__ uint32_t bytes() const { return hi > lo ? (uint32_t)(hi - lo) : 0u; }
+  __device__ __forceinline__ uint32_t bytes() const { return (uint32_t)(hi - lo); }
   __device__ __forceinline__ void go(uint32_t place, uint32_t bar) const {
-    if (hi > lo)
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                   ::"r"(place + (uint32_t)(lo - (begin & ~(uintptr_t)15))), "l"(lo), "r"((uint32_t)(hi - lo)), "r"(bar) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(place + (uint32_t)(lo - (begin & ~(uintptr_t)15))), "l"(lo), "r"(bytes()), "r"(bar) : "memory");
   }
 };
 template <class ROWS, int I>
@@ -502,14 +502,13 @@ __device__ __forceinline__ RingCopy ring_copy(const ROWS& rows, int row, int wid
   copy.hi = end & ~(uintptr_t)15;
   return copy;
 }
-// The elements outside that copy, by the lanes of a warp: at most 7 (of 2 bytes) before and 7 behind, or 15 in all.
+// The elements outside that copy, by the lanes of a warp: at most 7 (of 2 bytes) before and 7 behind.
 template <class ROWS, int I>
 __device__ __forceinline__ void ring_edges(const ROWS& rows, int row, int width, unsigned char* place, int lane) {
   using T = typename ROWS::template From<I>;
   const RingCopy copy = ring_copy<ROWS, I>(rows, row, width);
   const int count = ROWS::length(width), size = (int)sizeof(T);
-  const int before = copy.hi > copy.lo ? (int)(copy.lo - copy.begin) / size : count;
-  const int behind = copy.hi > copy.lo ? count - (int)(copy.hi - copy.begin) / size : 0;
+  const int before = (int)(copy.lo - copy.begin) / size, behind = count - (int)(copy.hi - copy.begin) / size;
   const int i = lane < 16 ? lane : count - behind + lane - 16;
   if (lane < 16 ? lane < before : lane - 16 < behind)
     reinterpret_cast<T*>(place + (copy.begin & 15))[i] = reinterpret_cast<const T*>(copy.begin)[i];

@@ -507,9 +507,9 @@ template <class ROWS, int I>
 __device__ __forceinline__ void ring_edges(const ROWS& rows, int row, int width, unsigned char* place, int lane) {
   using T = typename ROWS::template From<I>;
   const RingCopy copy = ring_copy<ROWS, I>(rows, row, width);
-  const int count = ROWS::length(width), size = (int)sizeof(T);
-  const int before = (int)(copy.lo - copy.begin) / size, behind = count - (int)(copy.hi - copy.begin) / size;
-  const int i = lane < 16 ? lane : count - behind + lane - 16;
+  const uint32_t count = ROWS::length(width), size = sizeof(T);  // (unsigned: a signed division by 2 or 4 is not a shift)
+  const int before = (uint32_t)(copy.lo - copy.begin) / size, behind = count - (uint32_t)(copy.hi - copy.begin) / size;
+  const int i = lane < 16 ? lane : (int)count - behind + lane - 16;
   if (lane < 16 ? lane < before : lane - 16 < behind)
     reinterpret_cast<T*>(place + (copy.begin & 15))[i] = reinterpret_cast<const T*>(copy.begin)[i];
 }

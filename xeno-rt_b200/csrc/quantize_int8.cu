@@ -112,7 +112,8 @@ __device__ __forceinline__ void store_some(float* p, const float (&v)[VEC]) {
 }
 
 // The codes of VEC values y / scale, `inverse` being 1 / scale; all zero with `broken`.  EXACT: of the quotient as a 32-bit division
-// rounds it (the product with the inverse, corrected once by its remainder).  A row that is coded as it is needs that: its values
+// rounds it: the product with the inverse, corrected once by its remainder (Markstein's correction: IBM J. Res. Dev. 34, 1990; of
+// bfloat16 values every such quotient is tested).  A row that is coded as it is needs that: its values
 // have few bits, and quotients in the middle between two codes, which go to the even one, are many.  What was computed on
 // the way here is not exact in its last bit.
 template <int VEC, bool EXACT>
@@ -346,6 +347,9 @@ struct RowScaleOf {
   float factor, scale, inverse;
   bool broken;
 };
+// The exact quotients of store_codes need remainders that are no smaller than what 32 bits hold: rows whose scale is below
+// TINY_SCALE are divided as LIFT times themselves, which changes no quotient.
+constexpr float TINY_SCALE = 8.2718061e-25f, LIFT = 18446744073709551616.0f;  // 2^-80, 2^64
 template <class ROWS>
 __device__ __forceinline__ RowScaleOf scale_of(const ROWS& rows, int width, uint32_t bits, float squares) {
   RowScaleOf s;
@@ -360,9 +364,17 @@ __device__ __forceinline__ RowScaleOf scale_of(const ROWS& rows, int width, uint
 template <class ROWS, int VEC, int ITEMS, bool LOOSE = false>
 __device__ __forceinline__ void finish_row(int8_t* codes, float* scales, const ROWS& rows, int row, int width, int ld_codes, int stride,
                                            uint32_t bits, float squares, float (&v)[ITEMS][VEC]) {
-  const RowScaleOf s = scale_of(rows, width, bits, squares);
+  RowScaleOf s = scale_of(rows, width, bits, squares);
   if (threadIdx.x == 0) scales[row] = s.scale;
   int8_t* dst = codes + (size_t)row * ld_codes;
+  if (ROWS::EXACT && s.scale < TINY_SCALE) {
+    s.scale *= LIFT;
+    s.inverse = 1.0f / s.scale;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] *= LIFT;
+  }
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     const int c = (int)threadIdx.x * VEC + i * stride;
@@ -434,8 +446,13 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
   if constexpr (ITEMS > 0) {
     finish_row<ROWS, VEC, KEPT>(codes, scales, rows, row, width, ld_codes, stride, bits, squares, v);
   } else {
-    const RowScaleOf s = scale_of(rows, width, bits, squares);
+    RowScaleOf s = scale_of(rows, width, bits, squares);
     if (threadIdx.x == 0) scales[row] = s.scale;
+    const bool lifted = ROWS::EXACT && s.scale < TINY_SCALE;
+    if (lifted) {
+      s.scale *= LIFT;
+      s.inverse = 1.0f / s.scale;
+    }
     int8_t* dst = codes + (size_t)row * ld_codes;
     for (int c = (int)threadIdx.x * VEC; c < width; c += stride) {
       rows.template ahead<VEC>(c, width, w[0]);
@@ -444,6 +461,10 @@ quantize_int8_kernel(int8_t* __restrict__ codes, float* __restrict__ scales, ROW
       if constexpr (ROWS::NORMED) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[0][j] *= s.factor;
+      }
+      if (lifted) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[0][j] *= LIFT;
       }
       store_codes<VEC, ROWS::EXACT>(dst + c, v[0], s.scale, s.inverse, s.broken);
     }

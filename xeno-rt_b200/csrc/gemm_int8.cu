@@ -12,8 +12,8 @@
 //               for both): four a stage, each 32 bytes of K.
 //   warps 3-6   epilogue: each warp reads its 32 TMEM lanes (rows), 32 columns at a time, applies the scales and writes
 //               patches of 32 rows x 128 bytes to shared memory, which a TMA store takes (or a TMA reduction adds into the
-//               output), while the MMA warp fills the other accumulator.  Outputs whose rows do not begin every 16
-//               bytes are stored by the warp, a row of 32 columns at a time.
+//               output), while the MMA warp fills the other accumulator.  Outputs whose rows do not begin and end
+//               every 16 bytes are stored by the warp, a row of 32 columns at a time.
 // What bounds it: the tensor pipe, 93 percent of whose cycles are taken while a block runs (2,048 rows of 28,672 outputs, 4,096
 // inputs 145-150 us; 8,192 546, 3,527 TOP/s, until the power limit lowers the clock: 655 in a loop of seconds).  Products of one
 // wave of tiles are their walk over K and the ends: 512 rows of 4,096, 4,096 11.2 us, 333 of 5,003, 1,999 7.7 (of 5,008, 2,048,
@@ -341,7 +341,8 @@ int launch_gemm_int8_tiled(const Int8Product& p, cudaStream_t stream) {
   CUtensorMap map_x, map_w, map_out = {};
   if (!make_map_int8_2d(&map_x, p.codes, p.M, p.K, p.ldx, I8_BM) || !make_map_int8_2d(&map_w, p.w, p.N, p.K, p.ldw, Shape::B_ROWS))
     return XRT_ERR_UNSUPPORTED;
-  const int by_tma = ((uintptr_t)p.out & 15) == 0 && (size_t)p.ldo * sizeof(TO) % 16 == 0;
+  // A TMA store writes whole pieces of 16 bytes: what a row's last one has beyond N would be overwritten with zeros.
+  const int by_tma = (((uintptr_t)p.out | (size_t)p.ldo * sizeof(TO) | (size_t)p.N * sizeof(TO)) & 15) == 0;
   if (by_tma && !make_map_result_2d(&map_out, p.out, p.M, p.N, p.ldo, sizeof(TO))) return XRT_ERR_UNSUPPORTED;
   constexpr int tile_rows = (PAIR ? 2 : 1) * I8_BM;
   const long long tiles = (long long)((p.M + tile_rows - 1) / tile_rows) * ((p.N + BN - 1) / BN);

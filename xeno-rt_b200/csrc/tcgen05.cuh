@@ -80,7 +80,8 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
 }
 
 // A tile of shared memory into a two-dimensional tensor map (or, with `add`, added into it, float32), in a group of this thread's;
-// writes of the tile by other threads must have been fenced (fence_to_async) before.  c0 as for the loads.
+// writes of the tile by other threads must have been fenced (fence_to_async) before.  c0 as for the loads.  Rows of the map end at
+// 16-byte boundaries too: what the last 16 bytes of a row hold beyond the map is overwritten with zeros (measured).
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src, bool add) {
   if (add)
     asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];"

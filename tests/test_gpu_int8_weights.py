@@ -53,3 +53,26 @@ def test_a_matrix_is_not_laid_out_inside_a_capture():
         product(out, x, matrix, False)  # which the refusal left as it was
     graph.replay()
     assert torch.equal(out, want)
+
+
+def test_memory_while_a_model_is_loaded(tmp_path):
+    """The whole model in the compute dtype, then part by part in 8 bits: the peak is the former and no more than the codes of
+    one layer, whose matrices are given up when all of its parts are laid out; what is left is less."""
+    from helpers import CONFIGS
+    from xeno_rt_b200 import write_random_model
+    from xeno_rt_b200.engine import Model
+    raw = dict(CONFIGS["tiny-wide"][0], hidden_size=1024, intermediate_size=4096, num_hidden_layers=6)
+    folder = str(tmp_path / "m")
+    write_random_model(folder, raw, 1, "bfloat16")
+    left, peak = {}, {}
+    for weights in (None, "int8"):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        model = Model.load(folder, dtype="bfloat16", weights=weights)
+        torch.cuda.synchronize()
+        left[weights], peak[weights] = torch.cuda.memory_allocated() - before, torch.cuda.max_memory_allocated() - before
+        del model
+    layer = 3 * 1024 * 4096 + 1024 * (raw["num_attention_heads"] + raw["num_key_value_heads"]) * raw["head_dim"] * 2  # bytes of codes
+    assert left["int8"] < left[None] - 0.9 * 6 * layer
+    assert peak["int8"] <= peak[None] + 1.1 * layer

@@ -46,3 +46,13 @@ def test_the_launchers_refuse_them_too():
     for m, n in ((o.INT8_MAX_SIZE + 1, 1), (1, o.INT8_MAX_SIZE + 1)):
         call = o._pack_int8_product(16, 16, 16, 16, 16, 0, 0, m, n, 16, 16, 16, n, 0, 0, 0)
         assert o.library().xrt_gemm_int8(call, 0) == -1
+
+
+def test_the_option_says_that_the_products_inputs_are_rounded_too(capsys):
+    from xeno_rt_b200.cli import build_parser
+    from xeno_rt_b200.engine.runtime import Runtime
+    with pytest.raises(SystemExit):
+        build_parser().parse_args(["generate", "--help"])
+    said = " ".join(capsys.readouterr().out.split())
+    assert "round the inputs of their products to 8 bits too" in said
+    assert "inputs of their products" in " ".join(Runtime.load.__doc__.split())

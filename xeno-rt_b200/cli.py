@@ -46,7 +46,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--seed", type=int, default=None)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     g.add_argument("--weights", default=None, choices=["int8"],
-                   help="hold attention's and the feed-forwards' matrices in 8 bits (default: in --dtype)")
+                   help="hold attention's and the feed-forwards' matrices in 8 bits, and round the inputs of their products "
+                        "to 8 bits too, a scale a row (default: both in --dtype)")
     g.add_argument("--stop-ids", type=_ids, default=None,
                    help="ids that end a sequence (default: eos_token_id of config.json)")
     g.add_argument("--device", default="cuda:0")

@@ -37,7 +37,9 @@ def check_weights_format(spec: ModelSpec, weights: str | None) -> None:
 class Model:
     def __init__(self, spec: ModelSpec, tensors: dict, dtype: DType, device, config=None, weights: str | None = None):
         """``weights`` = "int8": the matrices of attention and feed-forwards are held in 8 bits with a scale a row, and their
-        products run on 8-bit integers (parts/int8.py); ``tensors`` then gives each up once it has been laid out."""
+        products run on 8-bit integers (parts/int8.py), so that their inputs (the norms' results, attention's, the gates') are
+        rounded to 8 bits a row too, and the sums that enter a gate to the compute dtype; ``tensors`` gives each matrix up
+        once it has been laid out: until then the model takes the memory that it takes without."""
         ops.require_device()
         spec.validate()
         check_weights_format(spec, weights)
@@ -106,7 +108,8 @@ class Model:
     @classmethod
     def load(cls, folder: str, dtype="bfloat16", device="cuda:0", weights: str | None = None) -> "Model":
         """From a folder with config.json and model.safetensors; the model class is chosen by
-        config.json's architecture name.  ``weights``: None, or "int8" (see ``__init__``)."""
+        config.json's architecture name.  ``weights``: None, or "int8" (see ``__init__``): the tensors are loaded as they are
+        without first, and laid out part by part."""
         ops.require_device()
         dtype = parse_dtype(dtype)
         arch, config = load_config(folder)

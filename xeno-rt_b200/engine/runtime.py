@@ -108,7 +108,8 @@ class Runtime:
     @classmethod
     def load(cls, path: str, dtype="bfloat16", device="cuda:0", cache_tokens: int | None = None,
              max_batch: int = 64, weights: str | None = None) -> "Runtime":
-        """``weights`` = "int8": attention's and the feed-forwards' matrices in 8 bits (``Model``)."""
+        """``weights`` = "int8": attention's and the feed-forwards' matrices are held in 8 bits, and the inputs of their products
+        are rounded to 8 bits too, with a scale a row (``Model``)."""
         return cls(Model.load(path, dtype=dtype, device=device, weights=weights), cache_tokens, max_batch)
 
     def new_session(self) -> "Session":

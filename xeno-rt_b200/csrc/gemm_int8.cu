@@ -15,7 +15,7 @@
 //               output), while the MMA warp fills the other accumulator.  Outputs whose rows do not begin and end
 //               every 16 bytes are stored by the warp, a row of 32 columns at a time.
 // What bounds it: the tensor pipe, 93 percent of whose cycles are taken while a block runs (2,048 rows of 28,672 outputs, 4,096
-// inputs 145-150 us; 8,192 546, 3,527 TOP/s, until the power limit lowers the clock: 655 in a loop of seconds).  Products of one
+// inputs 145-153 us; 8,192 546, 3,527 TOP/s, until the power limit lowers the clock: 655 in a loop of seconds).  Products of one
 // wave of tiles are their walk over K and the ends: 512 rows of 4,096, 4,096 11.2 us, 333 of 5,003, 1,999 7.7 (of 5,008, 2,048,
 // whose output rows begin every 16 bytes, 7.2).  Few rows: see there.
 //
@@ -418,9 +418,10 @@ int launch_gemm_int8(const Int8Product& p, int form, cudaStream_t stream) {
 // kernel this short also pays for every instruction that it meets for the first time (its code comes from the L2): the
 // finish is one short loop, and while warps 5-8 wait they walk it once into a place that nobody reads.
 //
-// Measured on a B200, operands from memory, microseconds, the weight constant (bytes at 6.55 TB/s): 1 row of 6,144 outputs, 4,096
-// inputs 7.3 (3.9), 8 of 4,096, 14,336 12.3 (9.0), of 28,672, 4,096 19.6 (18.1), of 51,200, 5,120 39.4 (40.3), 64 of 28,672, 4,096
-// 21.8 (18.5), 128 of it 28.3 (20.2).  With a weight that may have just been written 0.2 to 0.9 more.
+// Measured on a B200, operands from memory, microseconds, the weight constant (its bytes and the codes' at the copy rate of 6.55 TB/s,
+// which reads alone may pass): 1 row of 6,144 outputs, 4,096 inputs 7.3 (3.9), 8 of 4,096, 14,336 12.3 (9.0), of 28,672,
+// 4,096 20.0 (18.1), of 51,200, 5,120 40.4 (40.3), 64 of 28,672, 4,096 21.9 (18.5).  With a weight that may have just been written 0.2
+// to 1.2 more.
 constexpr int FEW_MAX_ROWS = 128, FEW_MAX_SPLITS = 4, FEW_MAX_STAGES = 24;
 constexpr int FEW_PRODUCERS = 4;  // (the walk below counts on four)
 constexpr int FEW_THREADS = 32 * (FEW_PRODUCERS + 1 + 4);

@@ -7,20 +7,20 @@
 // every product with it is NaN.  Sums, statistics and y are 32-bit; the codes are the only rounding to fewer bits.
 //
 // One block a row, the row in registers: read once, one meeting of the block (the norm's sum of squares and the largest |s w|
-// are found in the same pass, since the factor 1 / rms is the same for the whole row), codes written once.  The largest absolute value is found on the bits: for numbers without
-// a sign their order is that of the integers, and every NaN lies above infinity.
+// are found in the same pass, since the factor 1 / rms is the same for the whole row), codes written once.  The largest absolute
+// value is found on the bits: for numbers without a sign their order is that of the integers, and every NaN lies above infinity.
 //
 // Few rows (steps): a block a row, its loads all in flight together.  More rows than blocks: blocks take every so many-th
 // row from a ring in shared memory that bulk copies fill ahead (quantize_int8_ring_kernel), so that the memory is asked for the
 // next rows while a block meets.  Rows beyond what 1,024 threads hold are walked twice.
 //
 // What bounds it: many long rows the memory, and beside it the instructions that a multiprocessor issues (hence Two, largest_of
-// and sigmoid below: gates 64 -> 51 us, 4,096 plain rows of 8,192 22.6 -> 20.6); few rows the time of one load, one meeting and
-// one store.  Measured on a B200, operands from memory, microseconds (bytes that it cannot do without at 6.55 TB/s): norm after
-// an addition of 1 row of 4,096 2.2, of 2,048 16.3 (14.1), of 8,191 of 5,120, float32 79-86 (83); gate of 8 rows of 14,336
-// units 2.8, of 2,048 29.6 (22.4), of 2,000 of 25,600 51 (39); plain rows, 64 of 4,096 1.5, 4,096 of 8,192 20.7 (15.4).
-// Rows of a width or an address that allows single values only take longer: norm of 2,047 of 4,095 36 (16.6), gates of 2,000 of
-// 25,599 75 (39).
+// and four_sigmoid below: gates 64 -> 51 us, 4,096 plain rows of 8,192 22.6 -> 20.6); few rows the time of one load, one meeting and
+// one store.  Measured on a B200, operands from memory, microseconds (bytes that it cannot do without at the copy rate of 6.55
+// TB/s): norm after an addition of 1 row of 4,096 2.2, of 2,048 16.2 (14.1), of 8,191 of 5,120, float32 79-87 (83), without one of
+// 2,048 of 4,096 10.4 (6.4); gate of 8 rows of 14,336 units 2.75, of 2,048 29.8 (22.4), of 2,000 of 25,600 52 (39); plain rows, 64
+// of 4,096 1.5, 2,000 6.9 (3.8), 4,096 of 8,192 20.8 (15.4).  Rows of a width or an address that allows single values only take
+// longer: norm of 2,047 of 4,095 35 (16.6), gates of 2,000 of 25,599 75 (39).
 #include <stddef.h>
 
 #include <type_traits>
@@ -170,7 +170,9 @@ struct PlainRows {
   static constexpr int early = 0;
   __device__ __forceinline__ void wait() { pdl_wait(x); }
   // the values from a row's streams where those lie in shared memory
-  template <int VEC, class READ> __device__ __forceinline__ void read(int c, int, const READ& get, float (&v)[VEC]) const { get.template operator()<0, VEC>(c, v); }
+  template <int VEC, class READ> __device__ __forceinline__ void read(int c, int, const READ& get, float (&v)[VEC]) const {
+    get.template operator()<0, VEC>(c, v);
+  }
   template <int VEC, bool LOOSE = false> __device__ __forceinline__ void ahead(int, int, float (&)[VEC]) const {}
   template <int VEC, bool AGAIN> __device__ __forceinline__ void load(int row, int c, int width, float (&v)[VEC]) const {
     load_some<VEC>(x + (size_t)row * width + c, v);
@@ -573,7 +575,10 @@ quantize_int8_ring_kernel(int8_t* __restrict__ codes, float* __restrict__ scales
   const int stride = (int)blockDim.x * VEC, stage_bytes = ring_stage<ROWS>(width), room0 = ring_room<ROWS, 0>(width);
   const int lane = threadIdx.x & 31;
   __syncthreads();
-  // A thread has the same columns of every row: it keeps their weights, where they leave room for the values.
+  // A thread has the same columns of every row: it keeps their weights, where they leave room for the values.  Microseconds, kept /
+  // read again for every row: without an addition 2,048 rows of 8,192 16.8 / 18.9, 8,191 of 14,336 90 / 110; with one, 600 of
+  // 8,192, float32 15.0 / 17.1, 2,048 39 / 41, 4,096 75 / 75.5, 8,191 153.6 / 147, and of 14,336, bfloat16 600 20.8 / 22.8, 4,096 115 /
+  // 112.5, 8,191 226 / 215: thousands of long rows with an addition lose 2 to 5 percent by it, fewer gain 5 to 13.
   constexpr bool KEEPS = ROWS::NORMED && VEC * ITEMS <= 16;
   float kept[KEEPS ? ITEMS : 1][VEC];
   auto keep = [&]() {
@@ -678,8 +683,8 @@ template <class ROWS, int VEC, int PER, bool LOOSE = false>
 int launch_quantize_ring(int8_t* codes, float* scales, const ROWS& rows, int n, int width, int ld_codes, int* error_flag,
                          cudaStream_t stream, bool& taken) {
   // Single values, but codes that allow pieces of four: four neighbours a thread, read one by one.  Microseconds, so / single
-  // values: 2,000 gates of 25,599 units 75 / 208, 600 of 5,003 7.9 / 13.2; 4,000 plain rows of 4,001 17.6 / 26.4;
-  // 2,047 norms of 4,095 16.5 / 18.6.  With an addition (whose sums would be written in parts of 32 bytes) 8,191 of 4,097 185 / 119, and
+  // values: 2,000 gates of 25,599 units 75 / 208, 600 of 5,003 7.9 / 13.2; 4,000 plain rows of 4,001 17.2 / 26.4;
+  // 2,047 norms of 4,095 16.5 / 18.6.  With an addition (whose sums would be written in parts of 32 bytes) 8,191 of 4,097 185 / 117, and
   // single values stay.
   if constexpr (VEC == 1 && ROWS::STREAMS == 1)
     if (((uintptr_t)codes | (uintptr_t)ld_codes) % 4 == 0)

@@ -1,9 +1,9 @@
 // The Blackwell (sm_100a) instructions that the tensor-core kernels of this library share, as thin
 // wrappers over inline PTX: mbarriers with bounded waits, TMA tensor copies, shared-memory and
 // instruction descriptors of tcgen05.mma (kind::f16, bfloat16 operands, float32 accumulators in tensor
-// memory; kind::i8, 8-bit and 32-bit integers), commits, fences, tensor-memory loads and stores, and the driver's tensor-map encoder.
-// Used by gemm_tcgen05.cu (prompt products), gemm_decode_tcgen05.cu (few-row products), gemm_int8.cu (8-bit products), moe_grouped.cu (experts'
-// products) and attention_prefill_tcgen05.cu (prompt attention).
+// memory; kind::i8, 8-bit and 32-bit integers), commits, fences, tensor-memory loads and stores, and the driver's
+// tensor-map encoder.  Used by gemm_tcgen05.cu (prompt products), gemm_decode_tcgen05.cu (few-row products), gemm_int8.cu (8-bit
+// products), moe_grouped.cu (experts' products) and attention_prefill_tcgen05.cu (prompt attention).
 #pragma once
 
 #include <cuda.h>

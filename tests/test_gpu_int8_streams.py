@@ -39,8 +39,9 @@ def test_chains_of_short_products_on_eight_streams(m, n, k):
         assert all(torch.equal(one, out) for out in got)
 
 
+@pytest.mark.parametrize("next_is_the_captures", [False, True])
 @pytest.mark.parametrize("mode", ["global", "thread_local", "relaxed"])
-def test_a_first_call_inside_a_capture_reports_its_errors_too(monkeypatch, mode):
+def test_a_first_call_inside_a_capture_reports_its_errors_too(monkeypatch, mode, next_is_the_captures):
     """The device's flag is made beside the capture: kernels of the graph get it, no replay clears it, and it is read as ever."""
     from xeno_rt_b200.core import KernelError
     from xeno_rt_b200.csrc import ops
@@ -53,6 +54,13 @@ def test_a_first_call_inside_a_capture_reports_its_errors_too(monkeypatch, mode)
     monkeypatch.setattr(ops, "_error_flags_at", {})
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, capture_error_mode=mode):
+        own = torch.cuda.current_stream().cuda_stream
+        if next_is_the_captures:  # the pool of streams is gone through until it gives the capture's again
+            taken = [torch.cuda.Stream().cuda_stream for _ in range(128)]
+            around = taken[::-1].index(taken[-1], 1)  # streams in the pool
+            place = taken[::-1].index(own)  # how many came after the capture's
+            for _ in range(around - 1 - place):
+                torch.cuda.Stream()
         ops.quantize_rows(codes, scales, x)
         inside = ops._error_flag_pointer(0)
     flag = ops._error_flags[0]

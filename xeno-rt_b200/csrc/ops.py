@@ -475,6 +475,11 @@ _error_flags: dict = {}
 _CAPTURE_RELAXED = 2  # cudaStreamCaptureModeRelaxed
 
 
+def _captures(stream) -> bool:
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def error_flag(device) -> torch.Tensor:
     """The int32 flag of ``device`` that kernels raise when a bounded wait inside them ran out.  Made when a model is built or at
     the first call that needs it; inside a stream capture beside the capture, on a stream of its own, so that it is no part of
@@ -487,6 +492,8 @@ def error_flag(device) -> torch.Tensor:
                 before = library().xrt_exchange_capture_mode(_CAPTURE_RELAXED)  # memory may be asked for beside the capture
                 try:
                     beside = torch.cuda.Stream()
+                    while _captures(beside):  # streams come from a pool, and the capture's is one of them
+                        beside = torch.cuda.Stream()
                     with torch.cuda.stream(beside):
                         flag = torch.zeros(1, dtype=torch.int32, device=device)
                     beside.synchronize()

@@ -83,3 +83,39 @@ def test_the_same_of_the_products_of_few_rows_in_bfloat16(tmp_path):
                     "-o", str(tmp_path / "main"), str(tmp_path / "main.cu")], check=True, capture_output=True, text=True)
     plans, bad, most = map(int, subprocess.run([str(tmp_path / "main")], check=True, capture_output=True, text=True).stdout.split())
     assert plans > 200 and most == 512 and bad == 0
+
+
+_SIZES = r"""
+#include <cuda_runtime.h>
+#include <cstdio>
+#include "gemm_tcgen05.cu"
+#include "gemm_int8.cu"
+namespace xrt { const Tuning& tuning() { static const Tuning t; return t; } }
+int main() {
+  printf("%d %d %d", xrt::TcShape<true>::SMEM, xrt::Int8Shape<true, 256>::SMEM, xrt::Int8Shape<true, 128>::SMEM);
+  return 0;
+}
+"""
+
+
+def test_no_block_with_tensor_memory_fits_beside_a_pair_that_has_all_of_it(tmp_path):
+    """Pairs of blocks take 512 columns in one multiprocessor and wait for as many in another: a block that fitted beside them could
+    hold what they wait for."""
+    from xeno_rt_b200.core import KernelError
+    from xeno_rt_b200.csrc import ops
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no nvcc")
+    try:
+        ops.library()
+    except KernelError as exc:
+        pytest.skip(f"the kernel library cannot be built here: {exc}")
+    (tmp_path / "main.cu").write_text(_SIZES)
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O0", "-Xcicc", "-O0", "-Xptxas", "-O0", "-std=c++17", "-I", CSRC,
+                    "-o", str(tmp_path / "main"), str(tmp_path / "main.cu")], check=True, capture_output=True, text=True)
+    bf16, all_columns, half = map(int, subprocess.run([str(tmp_path / "main")], check=True, capture_output=True, text=True).stdout.split())
+    least = min(p.shared_bytes for p in (ops.gemm_int8_plan(148, m, n, k) for m in (1, 16, 64, 128) for n in (1, 8, 600, 6144, 40000)
+                                         for k in (1, 128, 300, 4096)) if p.kernel == "few")
+    for pair in (bf16, all_columns):
+        assert pair + 1024 + least + 1024 > 228 * 1024
+    assert (half + 1024) * 512 >= 256 * 228 * 1024

@@ -21,7 +21,8 @@ constexpr int COPY_LIMIT = 1 << 14;  // 22 milliseconds: thousands of times what
 // a cluster.  An allocation waits until the multiprocessor has the columns to spare.  Two clusters that run at the same
 // time, each with one block that has its columns and one that waits for those which the other holds, would wait for ever.  So
 // columns are given out with shared memory: 456 of a multiprocessor's 233,472 bytes (1,024 of every block's share are the
-// system's) for each of its 512 columns, and blocks that fit one multiprocessor together always find theirs.
+// system's) for each of its 512 columns, and blocks that fit one multiprocessor together always find theirs.  (Pairs of blocks
+// with all 512 columns, of the products of many rows, leave 18 KB at most: no block that allocates any fits beside them.)
 __host__ __device__ constexpr int shared_bytes_of_columns(int columns) { return columns * 456 - 1024; }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
